@@ -379,6 +379,134 @@ int b2_adam_update(b2_stream_t stream, int num_tensors, float* const* params,
                    float one_minus_beta_1, float one_minus_beta_2,
                    float epsilon, int64_t* iterations, unsigned int* ticket);
 
+/* ---- Losses over rows of class scores --------------------------------------
+ * Not ops of the reference: the losses with which a network that ends in
+ * scores over many classes is trained on chosen classes, on another network's
+ * top answers, on pairs of answers or on rewards.
+ *
+ * Scores ("logits") are float32, float16 or bfloat16 rows of `classes`
+ * adjacent values; row (i, j), i < outer, j < inner, starts at element
+ * i * outer_stride + j * inner_stride of `data` (so the rows of a larger
+ * tensor, e.g. every position but the last of a batch of sequences, need no
+ * copy).  Rows are numbered i * inner + j; gradients of scores are dense
+ * [rows, classes] in the scores' type.  A class outside [0, classes) is
+ * ignored.  Integers are 32- or 64-bit as the *_bytes argument says (4, 8).
+ * Weights are null (all 1), float32 (4) or one byte each (1: 0 or not 0).  What
+ * belongs to a weight of 0 is not looked at.  A row of scores with a NaN or
+ * +inf, or with -inf only, has no softmax: its results are NaN (unless it
+ * does not count).  Results are deterministic.  Sums and softmax statistics
+ * are held in 32 bits or more. */
+
+typedef enum b2_dtype { B2_FLOAT32 = 0, B2_FLOAT16 = 1, B2_BFLOAT16 = 2 } b2_dtype_t;
+
+typedef struct b2_logits {
+  const void* data;
+  int32_t dtype; /* b2_dtype_t */
+  int64_t outer, inner, classes;
+  int64_t outer_stride, inner_stride; /* in elements */
+} b2_logits_t;
+
+/* log_probs[r] = x[r, t] - log sum_j exp(x[r, j]), t = targets[r]; 0 for an
+ * ignored target.  row_stats: [rows][2] floats for the gradient (the row's
+ * maximum m and sum_j exp(x_j - m)), or null. */
+int b2_token_log_probs(b2_stream_t stream, const b2_logits_t* logits,
+                       const void* targets, int target_bytes, float* log_probs,
+                       float* row_stats);
+
+/* grad_logits[r, j] = grad_log_probs[r] * ([j == t] - softmax(x[r])[j]); 0 for
+ * an ignored target or an upstream gradient of 0. */
+int b2_token_log_probs_grad(b2_stream_t stream, const b2_logits_t* logits,
+                            const void* targets, int target_bytes,
+                            const float* row_stats, const float* grad_log_probs,
+                            void* grad_logits);
+
+/* Distillation from a teacher's `top` (1 to 1024) entries per row: classes
+ * teacher_ids [rows, top] and their logits teacher_logits [rows, top].  With
+ * q[r] the softmax of the row's teacher logits / temperature over the entries
+ * whose class is not ignored and whose logit is not -inf, and P[r] the softmax
+ * of the row's scores / temperature over all classes:
+ *   l[r] = temperature^2 * sum_k q[r,k] (log q[r,k] - log P[r, id[r,k]])
+ *   *loss = sum_r w[r] l[r] / sum_r w[r]           (0 when the weights sum to 0)
+ * A class may be repeated in a row; l[r] = 0 for a row without entries.
+ * With grad_logits, the gradient too, in the same pass over the scores:
+ *   grad[r, j] = grad_loss * temperature * w[r] / sum w
+ *                * (P[r, j] - sum_{k: id[r,k] == j} q[r,k])
+ * grad_loss: a device float, or null for 1.  row_stats as above or null. */
+int b2_distillation_loss(b2_stream_t stream, const b2_logits_t* logits,
+                         const void* teacher_ids, int id_bytes,
+                         const void* teacher_logits, int teacher_dtype,
+                         int64_t top, const void* weights, int weight_bytes,
+                         double temperature, float* loss, float* row_stats,
+                         const float* grad_loss, void* grad_logits);
+
+/* The gradient alone, from the row_stats of b2_distillation_loss. */
+int b2_distillation_loss_grad(b2_stream_t stream, const b2_logits_t* logits,
+                              const void* teacher_ids, int id_bytes,
+                              const void* teacher_logits, int teacher_dtype,
+                              int64_t top, const void* weights,
+                              int weight_bytes, double temperature,
+                              const float* row_stats, const float* grad_loss,
+                              void* grad_logits);
+
+/* Preference loss over `pairs` pairs of token sequences.  offsets [2 pairs + 1],
+ * non-decreasing: sequence i is the tokens offsets[i] .. offsets[i+1] - 1,
+ * sequences 0 .. pairs-1 the chosen answers and pairs .. 2 pairs - 1 the rejected
+ * ones (offsets outside [0, tokens] are taken as the nearest of the two).
+ *   rewards[i] = beta * sum_n w[n] (log_probs[n] - ref_log_probs[n])
+ *   h[p] = rewards[p] - rewards[pairs + p]
+ *   *loss = mean_p -(1 - e) log sigma(h[p]) - e log sigma(-h[p]),
+ * e = label_smoothing in [0, 0.5]; ref_log_probs may be null (0).  slopes
+ * [2 pairs]: for the gradient. */
+int b2_preference_loss(b2_stream_t stream, const float* log_probs,
+                       const float* ref_log_probs, const void* weights,
+                       int weight_bytes, int64_t tokens, const void* offsets,
+                       int offset_bytes, int64_t pairs, double beta,
+                       double label_smoothing, float* loss, float* rewards,
+                       float* slopes);
+
+/* grad_log_probs[n] = *grad_loss * w[n] * slope of n's sequence; 0 for tokens in
+ * no sequence. */
+int b2_preference_loss_grad(b2_stream_t stream, const float* grad_loss,
+                            const float* slopes, const void* weights,
+                            int weight_bytes, int64_t tokens,
+                            const void* offsets, int offset_bytes,
+                            int64_t pairs, float* grad_log_probs);
+
+/* Clipped policy loss with a KL term over tokens, with A = advantages,
+ * r = exp(log_probs - old_log_probs), d = ref_log_probs - log_probs:
+ *   l = max(-r A, -clip(r, 1 - clip_low, 1 + clip_high) A)
+ *       + kl_coef (exp(d) - d - 1)                       (0 without ref_log_probs)
+ *   *loss = sum w l / sum w,            stats[0] = sum w (exp(d) - d - 1) / sum w,
+ *   stats[1] = share of the weight whose ratio is clipped (A > 0 and
+ *              r > 1 + clip_high, or A < 0 and r < 1 - clip_low),
+ *   stats[2] = 1 / sum w;               all 0 when the weights sum to 0.
+ * slopes [tokens]: for the gradient, or null. */
+int b2_policy_loss(b2_stream_t stream, const float* log_probs,
+                   const float* old_log_probs, const float* advantages,
+                   const float* ref_log_probs, const void* weights,
+                   int weight_bytes, int64_t tokens, double clip_low,
+                   double clip_high, double kl_coef, float* loss,
+                   float* stats, float* slopes);
+
+/* grad_log_probs = *grad_loss * stats[2] * slopes: d l / d log_probs is
+ * -A r where the ratio is not clipped, 0 where it is, + kl_coef (1 - exp(d)). */
+int b2_policy_loss_grad(b2_stream_t stream, const float* grad_loss,
+                        const float* stats, const float* slopes,
+                        int64_t tokens, float* grad_log_probs);
+
+/* b2_policy_loss of b2_token_log_probs(logits, targets), with the gradient of
+ * the scores, in one pass over them (stats has 2 elements here).  grad_loss: a
+ * device float, or null for 1. */
+int b2_policy_loss_with_grad(b2_stream_t stream, const b2_logits_t* logits,
+                             const void* targets, int target_bytes,
+                             const float* old_log_probs,
+                             const float* advantages,
+                             const float* ref_log_probs, const void* weights,
+                             int weight_bytes, double clip_low,
+                             double clip_high, double kl_coef,
+                             const float* grad_loss, float* loss, float* stats,
+                             void* grad_logits);
+
 /* Number of bounded device-side waits (tensor-core pipeline barriers) that
  * expired since the library was loaded; synchronise the stream first.  A
  * nonzero count means a kernel gave up waiting and its output is invalid. */

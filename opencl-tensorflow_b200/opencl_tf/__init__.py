@@ -18,7 +18,9 @@ OpenCLBatchNormalization, OpenCLReLU, OpenCLSigmoid, OpenCLDense,
 OpenCLUpSampling2D.
 
 Beyond the reference's op set: ``fused_ops`` (BatchNorm -> ReLU in one op),
-``step_ops`` (the MSE loss of the training recipe) and ``optimizers.Adam``
+``step_ops`` (the MSE loss of the training recipe), ``losses`` (losses over
+rows of class scores: log-probabilities of chosen classes, distillation,
+preferences, clipped policy) and ``optimizers.Adam``
 (Keras Adam as one multi-tensor kernel); ``train.TrainStep`` runs the whole
 training step from one CUDA graph.
 """
@@ -49,6 +51,7 @@ from .ops import (
 from . import errors  # noqa: F401
 from . import gradients  # noqa: F401  -- registers the gradient functions
 from . import layers  # noqa: F401
+from . import losses  # noqa: F401
 from . import optimizers  # noqa: F401
 
 __all__ = [
@@ -60,7 +63,7 @@ __all__ = [
     "sigmoid", "sigmoid_grad",
     "dense", "dense_backprop_input", "dense_backprop_weight", "dense_backprop_bias",
     "upsampling_bilinear_2d", "upsampling_bilinear_2d_grad",
-    "fused_ops", "step_ops", "optimizers",
+    "fused_ops", "step_ops", "losses", "optimizers",
     "layers", "errors", "init", "pool_stats", "pool_trim", "device_timeouts", "stream_status",
     "set_wait_limit_ns", "set_reserved_sms", "library_path",
 ]

@@ -28,6 +28,7 @@ import types
 from pathlib import Path
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import errors
 
@@ -46,6 +47,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _F32 = ctypes.c_float
+_F64 = ctypes.c_double
 _S = ctypes.c_char_p
 _I64x4 = _I64 * 4
 _I64x2 = _I64 * 2
@@ -84,6 +86,15 @@ _SIGS = {
     "b2_mse_loss": [_P, _P, _P, _I64, _P],
     "b2_mse_loss_grad": [_P, _P, _P, _I64, _P, _P],
     "b2_adam_update": [_P, _I, _P, _P, _P, _P, _P, _F32, _F32, _F32, _F32, _F32, _F32, _P, _P],
+    "b2_token_log_probs": [_P, _P, _P, _I, _P, _P],
+    "b2_token_log_probs_grad": [_P, _P, _P, _I, _P, _P, _P],
+    "b2_distillation_loss": [_P, _P, _P, _I, _P, _I, _I64, _P, _I, _F64, _P, _P, _P, _P],
+    "b2_distillation_loss_grad": [_P, _P, _P, _I, _P, _I, _I64, _P, _I, _F64, _P, _P, _P],
+    "b2_preference_loss": [_P, _P, _P, _P, _I, _I64, _P, _I, _I64, _F64, _F64, _P, _P, _P],
+    "b2_preference_loss_grad": [_P, _P, _P, _P, _I, _I64, _P, _I, _I64, _P],
+    "b2_policy_loss": [_P, _P, _P, _P, _P, _P, _I, _I64, _F64, _F64, _F64, _P, _P, _P],
+    "b2_policy_loss_grad": [_P, _P, _P, _P, _I64, _P],
+    "b2_policy_loss_with_grad": [_P, _P, _P, _I, _P, _P, _P, _P, _I, _F64, _F64, _F64, _P, _P, _P, _P],
     "b2_pool_trim": [],
     "b2_device_timeouts": [ctypes.POINTER(ctypes.c_uint)],
     "b2_stream_status": [_P],
@@ -107,6 +118,12 @@ for _name, _args in {"b2_peer_buffer_create": [ctypes.c_size_t, _VPP, _U8P],
                      "b2_peer_allreduce_avg": [_P, _P, _I64, _I, _I, _VPP, _P]}.items():
     getattr(_lib, _name).argtypes = _args
     getattr(_lib, _name).restype = _I
+
+
+class Logits(ctypes.Structure):
+    """``b2_logits_t``: rows of class scores."""
+    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("outer", _I64), ("inner", _I64),
+                ("classes", _I64), ("outer_stride", _I64), ("inner_stride", _I64)]
 
 
 class PoolStats(ctypes.Structure):
@@ -578,6 +595,237 @@ def _k_upsampling_bilinear2d_grad(grad_out, input_sizes, size):
     return dx
 
 
+# ------------------------------------------- losses over rows of class scores
+
+_FLOATS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # b2_dtype_t
+
+
+def _on_cuda(t, what: str) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise errors.InvalidArgumentError(f"{what} must be a torch tensor on a CUDA device")
+    if not t.is_cuda:
+        raise errors.InvalidArgumentError(
+            f"{what} must live on a CUDA device (this backend has no CPU path)")
+
+
+def _logits(t, what: str):
+    """(tensor, b2_logits_t) of scores [..., classes]; leading axes that fold
+    into two strides are read in place, others are copied."""
+    _on_cuda(t, what)
+    if t.dtype not in _FLOATS:
+        raise errors.InvalidArgumentError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    if t.dim() < 1 or t.shape[-1] < 1:
+        raise errors.InvalidArgumentError(f"{what} must be [..., classes] with at least one class")
+    classes = t.shape[-1]
+    if not t.is_contiguous():
+        axes = []  # (size, stride) of the leading axes, adjacent ones folded
+        for size, stride in zip(t.shape[:-1], t.stride()[:-1]):
+            if size == 1:
+                continue
+            if axes and axes[-1][1] == size * stride:
+                axes[-1] = (axes[-1][0] * size, stride)
+            else:
+                axes.append((size, stride))
+        if len(axes) <= 2 and (t.stride(-1) == 1 or classes == 1):
+            (outer, so), (inner, si) = [(1, 0)] * (2 - len(axes)) + axes
+            return t, Logits(t.data_ptr(), _FLOATS[t.dtype], outer, inner, classes, so, si)
+        t = t.contiguous()
+    return t, Logits(t.data_ptr(), _FLOATS[t.dtype], 1, t.numel() // classes, classes, 0, classes)
+
+
+def _same(t, what: str, shape, device, dtypes, names: str) -> torch.Tensor:
+    _on_cuda(t, what)
+    if t.dtype not in dtypes:
+        raise errors.InvalidArgumentError(f"{what} must be {names}, got {t.dtype}")
+    if t.shape != shape:
+        raise errors.InvalidArgumentError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise errors.InvalidArgumentError(f"{what} must live on {device}, got {t.device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+_INTS = (torch.int64, torch.int32)
+_WEIGHTS = (torch.float32, torch.bool, torch.uint8)
+
+
+def _ints(t, what, shape, device):
+    return _same(t, what, shape, device, _INTS, "int32 or int64")
+
+
+def _per_token(t, what, shape, device):
+    return None if t is None else _same(t, what, shape, device, (torch.float32,), "float32")
+
+
+def _weights(t, what, shape, device):
+    return None if t is None else _same(t, what, shape, device, _WEIGHTS, "float32, bool or uint8")
+
+
+def _scalar(t, what, device):
+    if t is None:
+        return None
+    _on_cuda(t, what)
+    if t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
+        raise errors.InvalidArgumentError(f"{what} must be a float32 scalar on {device}")
+    return t
+
+
+def _opt(t):
+    return None if t is None else t.data_ptr()
+
+
+def _size(t):
+    return 0 if t is None else t.element_size()
+
+
+def _f32(shape, device):
+    return torch.empty(shape, device=device, dtype=torch.float32)
+
+
+def _dense_like(x):
+    return torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+
+def _k_token_log_probs(logits, targets, with_stats=False):
+    x, v = _logits(logits, "logits")
+    t = _ints(targets, "targets", x.shape[:-1], x.device)
+    out = _f32(t.shape, x.device)
+    stats = _f32((*t.shape, 2), x.device) if with_stats else None
+    with _on_device(x):
+        _check(_lib.b2_token_log_probs(_stream(x), ctypes.byref(v), _p(t), t.element_size(), _p(out), _opt(stats)))
+    return (out, stats) if with_stats else out
+
+
+def _k_token_log_probs_grad(grad_log_probs, logits, targets, row_stats):
+    x, v = _logits(logits, "logits")
+    t = _ints(targets, "targets", x.shape[:-1], x.device)
+    g = _per_token(grad_log_probs, "grad_log_probs", t.shape, x.device)
+    st = _per_token(row_stats, "row_stats", (*t.shape, 2), x.device)
+    if g is None or st is None:
+        raise errors.InvalidArgumentError("grad_log_probs and row_stats must be torch tensors on a CUDA device")
+    out = _dense_like(x)
+    with _on_device(x):
+        _check(_lib.b2_token_log_probs_grad(_stream(x), ctypes.byref(v), _p(t), t.element_size(), _p(st), _p(g),
+                                            _p(out)))
+    return out
+
+
+def _teacher(x, teacher_ids, teacher_logits, weights):
+    lead = x.shape[:-1]
+    if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dim() != x.dim():
+        raise errors.InvalidArgumentError("teacher_ids must be [..., entries] with the leading axes of logits")
+    ids = _ints(teacher_ids, "teacher_ids", (*lead, teacher_ids.shape[-1]), x.device)
+    y = _same(teacher_logits, "teacher_logits", ids.shape, x.device, _FLOATS, "float32, float16 or bfloat16")
+    return ids, y, _weights(weights, "weights", lead, x.device)
+
+
+def _k_distillation_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0, with_stats=False,
+                         with_grad=False, grad_loss=None):
+    x, v = _logits(logits, "logits")
+    ids, y, w = _teacher(x, teacher_ids, teacher_logits, weights)
+    gl = _scalar(grad_loss, "grad_loss", x.device)
+    loss = _f32((), x.device)
+    stats = _f32((*x.shape[:-1], 2), x.device) if with_stats else None
+    grad = _dense_like(x) if with_grad else None
+    with _on_device(x):
+        _check(_lib.b2_distillation_loss(_stream(x), ctypes.byref(v), _p(ids), ids.element_size(), _p(y),
+                                         _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w), float(temperature),
+                                         _p(loss), _opt(stats), _opt(gl), _opt(grad)))
+    return (loss, stats) if with_stats else (loss, grad) if with_grad else loss
+
+
+def _k_distillation_loss_grad(logits, teacher_ids, teacher_logits, weights, temperature, row_stats, grad_loss):
+    x, v = _logits(logits, "logits")
+    ids, y, w = _teacher(x, teacher_ids, teacher_logits, weights)
+    gl = _scalar(grad_loss, "grad_loss", x.device)
+    st = _per_token(row_stats, "row_stats", (*x.shape[:-1], 2), x.device)
+    if gl is None or st is None:
+        raise errors.InvalidArgumentError("grad_loss and row_stats must be torch tensors on a CUDA device")
+    out = _dense_like(x)
+    with _on_device(x):
+        _check(_lib.b2_distillation_loss_grad(_stream(x), ctypes.byref(v), _p(ids), ids.element_size(), _p(y),
+                                              _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w),
+                                              float(temperature), _p(st), _p(gl), _p(out)))
+    return out
+
+
+def _offsets(offsets, device):
+    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 3 or offsets.numel() % 2 == 0:
+        raise errors.InvalidArgumentError("offsets must have 2 * pairs + 1 elements, pairs >= 1")
+    return _ints(offsets, "offsets", offsets.shape, device), offsets.numel() // 2
+
+
+def _k_preference_loss(log_probs, offsets, ref_log_probs=None, mask=None, beta=0.1, label_smoothing=0.0):
+    """-> loss, rewards [2 * pairs], slopes [2 * pairs]"""
+    lp = _input(log_probs, "log_probs")
+    off, pairs = _offsets(offsets, lp.device)
+    ref = _per_token(ref_log_probs, "ref_log_probs", lp.shape, lp.device)
+    w = _weights(mask, "mask", lp.shape, lp.device)
+    loss, rewards, slopes = _f32((), lp.device), _f32(2 * pairs, lp.device), _f32(2 * pairs, lp.device)
+    with _on_device(lp):
+        _check(_lib.b2_preference_loss(_stream(lp), _p(lp), _opt(ref), _opt(w), _size(w), lp.numel(), _p(off),
+                                       off.element_size(), pairs, float(beta), float(label_smoothing), _p(loss),
+                                       _p(rewards), _p(slopes)))
+    return loss, rewards, slopes
+
+
+def _k_preference_loss_grad(grad_loss, slopes, offsets, mask, shape):
+    device = slopes.device
+    gl = _scalar(grad_loss, "grad_loss", device)
+    off, pairs = _offsets(offsets, device)
+    sl = _per_token(slopes, "slopes", (2 * pairs,), device)
+    w = _weights(mask, "mask", shape, device)
+    out = _f32(shape, device)
+    with _on_device(out):
+        _check(_lib.b2_preference_loss_grad(_stream(out), _p(gl), _p(sl), _opt(w), _size(w), out.numel(), _p(off),
+                                            off.element_size(), pairs, _p(out)))
+    return out
+
+
+def _policy_inputs(shape, device, old_log_probs, advantages, ref_log_probs, mask):
+    old = _per_token(old_log_probs, "old_log_probs", shape, device)
+    adv = _per_token(advantages, "advantages", shape, device)
+    if old is None or adv is None:
+        raise errors.InvalidArgumentError("old_log_probs and advantages must be torch tensors on a CUDA device")
+    return old, adv, _per_token(ref_log_probs, "ref_log_probs", shape, device), _weights(mask, "mask", shape, device)
+
+
+def _k_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs=None, mask=None, clip_low=0.2, clip_high=0.2,
+                   kl_coef=0.0, with_slopes=False):
+    """-> loss, stats (mean KL, clipped share, 1 / sum of the weights), slopes or None"""
+    lp = _input(log_probs, "log_probs")
+    old, adv, ref, w = _policy_inputs(lp.shape, lp.device, old_log_probs, advantages, ref_log_probs, mask)
+    loss, stats = _f32((), lp.device), _f32(3, lp.device)
+    slopes = _f32(lp.shape, lp.device) if with_slopes else None
+    with _on_device(lp):
+        _check(_lib.b2_policy_loss(_stream(lp), _p(lp), _p(old), _p(adv), _opt(ref), _opt(w), _size(w), lp.numel(),
+                                   float(clip_low), float(clip_high), float(kl_coef), _p(loss), _p(stats),
+                                   _opt(slopes)))
+    return loss, stats, slopes
+
+
+def _k_policy_loss_grad(grad_loss, stats, slopes):
+    gl = _scalar(grad_loss, "grad_loss", slopes.device)
+    out = torch.empty_like(slopes)
+    with _on_device(out):
+        _check(_lib.b2_policy_loss_grad(_stream(out), _p(gl), _p(stats), _p(slopes), out.numel(), _p(out)))
+    return out
+
+
+def _k_policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs=None, mask=None, clip_low=0.2,
+                             clip_high=0.2, kl_coef=0.0, grad_loss=None):
+    """-> loss, stats (mean KL, clipped share), grad_logits"""
+    x, v = _logits(logits, "logits")
+    t = _ints(targets, "targets", x.shape[:-1], x.device)
+    old, adv, ref, w = _policy_inputs(t.shape, x.device, old_log_probs, advantages, ref_log_probs, mask)
+    gl = _scalar(grad_loss, "grad_loss", x.device)
+    loss, stats, grad = _f32((), x.device), _f32(2, x.device), _dense_like(x)
+    with _on_device(x):
+        _check(_lib.b2_policy_loss_with_grad(_stream(x), ctypes.byref(v), _p(t), t.element_size(), _p(old), _p(adv),
+                                             _opt(ref), _opt(w), _size(w), float(clip_low), float(clip_high),
+                                             float(kl_coef), _opt(gl), _p(loss), _p(stats), _p(grad)))
+    return loss, stats, grad
+
+
 # ------------------------------------------------------- gradient registry
 
 _GRADIENTS: dict = {}
@@ -644,6 +892,80 @@ def _apply(op_type: str, kernel, inputs, attrs, nondiff=()):
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
         return _OpNode.apply(op_type, attrs, kernel, tuple(nondiff), *inputs)
     return kernel(*inputs, **attrs)
+
+
+# The losses' gradients need more than an op's inputs and outputs (the rows'
+# softmax statistics, the slopes of sequences and tokens), so each is an
+# autograd node of its own instead of a registered gradient function.
+
+class _TokenLogProbsNode(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets):
+        out, stats = _k_token_log_probs(logits, targets, with_stats=True)
+        ctx.save_for_backward(logits, targets, stats)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        logits, targets, stats = ctx.saved_tensors
+        return _k_token_log_probs_grad(grad, logits, targets, stats), None
+
+
+class _DistillationNode(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_ids, teacher_logits, weights, temperature):
+        loss, stats = _k_distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature, with_stats=True)
+        ctx.save_for_backward(logits, teacher_ids, teacher_logits, weights, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        logits, ids, y, weights, stats = ctx.saved_tensors
+        return _k_distillation_loss_grad(logits, ids, y, weights, ctx.temperature, stats, grad), None, None, None, None
+
+
+class _PreferenceNode(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, log_probs, offsets, ref_log_probs, mask, beta, label_smoothing):
+        loss, rewards, slopes = _k_preference_loss(log_probs, offsets, ref_log_probs, mask, beta, label_smoothing)
+        ctx.save_for_backward(offsets, mask, slopes)
+        ctx.shape = log_probs.shape
+        ctx.mark_non_differentiable(rewards)
+        ctx.set_materialize_grads(False)
+        return loss, rewards
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _grad_rewards):
+        if grad is None:
+            return (None,) * 6
+        offsets, mask, slopes = ctx.saved_tensors
+        return _k_preference_loss_grad(grad, slopes, offsets, mask, ctx.shape), None, None, None, None, None
+
+
+class _PolicyNode(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low, clip_high, kl_coef):
+        loss, stats, slopes = _k_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low,
+                                             clip_high, kl_coef, with_slopes=True)
+        ctx.save_for_backward(stats, slopes)
+        ctx.mark_non_differentiable(stats)
+        ctx.set_materialize_grads(False)
+        return loss, stats
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _grad_stats):
+        if grad is None:
+            return (None,) * 8
+        return (_k_policy_loss_grad(grad, *ctx.saved_tensors),) + (None,) * 7
+
+
+def _differentiable(t) -> bool:
+    return isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled()
 
 
 # --------------------------------------------------------------- raw_ops
@@ -784,14 +1106,53 @@ def _mk_step_ops():
     def opencl_mse_loss_grad(y_pred, y_true, grad_loss):
         return _k_mse_loss_grad(y_pred, y_true, grad_loss)
 
-    ns.opencl_mse_loss = _traced("opencl_mse_loss", opencl_mse_loss)
-    ns.opencl_mse_loss_grad = _traced("opencl_mse_loss_grad", opencl_mse_loss_grad)
+    def opencl_token_log_probs(logits, targets):
+        if _differentiable(logits):
+            return _TokenLogProbsNode.apply(logits, targets)
+        return _k_token_log_probs(logits, targets)
+
+    def opencl_distillation_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0):
+        if _differentiable(logits):
+            return _DistillationNode.apply(logits, teacher_ids, teacher_logits, weights, float(temperature))
+        return _k_distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature)
+
+    def opencl_distillation_loss_with_grad(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0,
+                                           grad_loss=None):
+        return _k_distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature, with_grad=True,
+                                    grad_loss=grad_loss)
+
+    def opencl_preference_loss(log_probs, offsets, ref_log_probs=None, mask=None, beta=0.1, label_smoothing=0.0):
+        """-> loss, rewards of the 2 * pairs sequences"""
+        if _differentiable(log_probs):
+            return _PreferenceNode.apply(log_probs, offsets, ref_log_probs, mask, float(beta), float(label_smoothing))
+        return _k_preference_loss(log_probs, offsets, ref_log_probs, mask, beta, label_smoothing)[:2]
+
+    def opencl_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs=None, mask=None, clip_low=0.2,
+                           clip_high=0.2, kl_coef=0.0):
+        """-> loss, stats (mean KL, clipped share, 1 / sum of the weights)"""
+        if _differentiable(log_probs):
+            return _PolicyNode.apply(log_probs, old_log_probs, advantages, ref_log_probs, mask, float(clip_low),
+                                     float(clip_high), float(kl_coef))
+        return _k_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low, clip_high,
+                              kl_coef)[:2]
+
+    def opencl_policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs=None, mask=None,
+                                     clip_low=0.2, clip_high=0.2, kl_coef=0.0, grad_loss=None):
+        """-> loss, stats (mean KL, clipped share), grad_logits"""
+        return _k_policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs, mask, clip_low,
+                                        clip_high, kl_coef, grad_loss)
+
+    for k, v in list(locals().items()):
+        if k.startswith("opencl_"):
+            setattr(ns, k, _traced(k, v))
     return ns
 
 
 step_ops = _mk_step_ops()
-"""The training step's loss on the device: stock Keras in the reference
-(``model.compile(loss="mse")``, README.md:188-196), not an op of its library."""
+"""The training step's losses on the device.  The mean squared error is stock
+Keras in the reference (``model.compile(loss="mse")``, README.md:188-196), not an
+op of its library; the losses over rows of class scores have no counterpart
+there (``losses.py`` documents them)."""
 
 
 # ------------------------------------------------------- runtime utilities
