@@ -1,0 +1,121 @@
+// log_prob_common.cuh -- what the losses over rows of class scores share between
+// the row kernels (one source file for each type of score) and the entries.
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "b2_internal.cuh"
+
+namespace b2 {
+
+enum Mode { kLogProb = 0, kDistill = 1, kPolicy = 2 };
+
+struct PolicyToken {
+  float old_lp, advantage, ref_lp;
+  bool has_ref;
+};
+struct PolicyClip {
+  double low, high;  // the ratio's range
+  float kl_coef;
+};
+struct RowArgs {
+  const void* x;
+  int64_t rows, inner, outer_stride, inner_stride;
+  int classes;
+  int slice;          // values of a row that each CTA of a cluster has, a multiple of 8
+  int filter_words;   // of each of a teacher's two bit filters, a power of two
+  int teacher_bytes;  // shared memory of a row's teacher
+  float c;  // log2(e) / temperature
+  float temperature, inv_t;
+  float2* stats;   // [rows] (m, s): written by pass 1 unless null, read by pass 2 alone
+  void* grad;      // [rows, classes] dense; null: no pass 2
+  // the chosen classes
+  const void* ids;
+  int ids_bytes, top;
+  const void* teacher;
+  int teacher_dtype;
+  // what multiplies a row
+  const void* weights;  // null: 1; float, or one byte a row (0 / not 0)
+  int weight_bytes;
+  const double* total;     // sum of the weights; null: rows
+  const float* upstream;   // per row (log-probability gradient)
+  const float* grad_loss;  // scalar; null: 1
+  // policy
+  const float *old_lp, *ref_lp, *advantages;
+  PolicyClip clip;
+  // results per row
+  float* log_probs;
+  double* row_out;  // [1 or 3][rows], multiplied by the row's weight
+};
+
+// The passes over the rows: pass 1 (statistics, and the loss of each row) when
+// `stats`, pass 2 (the gradient) when `grad`.
+int launch_rows_f32(cudaStream_t s, const RowArgs& a, Mode mode, bool stats, bool grad, const DeviceInfo* d,
+                    const char* what);
+int launch_rows_f16(cudaStream_t s, const RowArgs& a, Mode mode, bool stats, bool grad, const DeviceInfo* d,
+                    const char* what);
+int launch_rows_bf16(cudaStream_t s, const RowArgs& a, Mode mode, bool stats, bool grad, const DeviceInfo* d,
+                     const char* what);
+
+constexpr int kMaxTop = 1024;  // teacher entries of a row
+
+__device__ __forceinline__ int64_t class_at(const void* ids, int bytes, int64_t i) {
+  return bytes == 8 ? static_cast<const int64_t*>(ids)[i] : (int64_t) static_cast<const int32_t*>(ids)[i];
+}
+
+__device__ __forceinline__ float weight_at(const void* w, int bytes, int64_t i) {
+  if (w == nullptr) return 1.0f;
+  return bytes == 4 ? static_cast<const float*>(w)[i] : (static_cast<const uint8_t*>(w)[i] != 0 ? 1.0f : 0.0f);
+}
+
+struct PolicyTerm {
+  float value, slope, kl;
+  bool cut;
+};
+
+// One token's term of the clipped policy loss and its slope in the token's
+// log-probability, in 32 bits.  Only a ratio within 1e-5 of a border, where its
+// rounding could put it on the other side, is looked at again in 64; and
+// exp(d) - d - 1 is its series for |d| <= 1, where the subtraction would cancel.
+__device__ __forceinline__ PolicyTerm policy_term(float lp, const PolicyToken& t, const PolicyClip& c) {
+  PolicyTerm p;
+  const float low = (float)c.low, high = (float)c.high, adv = t.advantage;
+  const float ratio = expf(lp - t.old_lp);
+  bool above = ratio > high, below = ratio < low;
+  if (fabsf(ratio - high) <= 1e-5f * high || fabsf(ratio - low) <= 1e-5f) {
+    const double exact = exp((double)lp - (double)t.old_lp);
+    above = exact > c.high;
+    below = exact < c.low;
+  }
+  p.cut = (adv > 0.0f && above) || (adv < 0.0f && below);
+  // Where it is not cut, the unclipped term is the larger one.
+  p.value = p.cut ? -(above ? high : low) * adv : -ratio * adv;
+  p.slope = p.cut ? 0.0f : -adv * ratio;
+  p.kl = 0.0f;
+  if (t.has_ref) {
+    const float d = t.ref_lp - lp;
+    if (fabsf(d) <= 1.0f) {
+      float s = 1.0f / 39916800.0f;  // sum of d^(k - 2) / k!, k = 2 .. 11
+      s = fmaf(s, d, 1.0f / 3628800.0f);
+      s = fmaf(s, d, 1.0f / 362880.0f);
+      s = fmaf(s, d, 1.0f / 40320.0f);
+      s = fmaf(s, d, 1.0f / 5040.0f);
+      s = fmaf(s, d, 1.0f / 720.0f);
+      s = fmaf(s, d, 1.0f / 120.0f);
+      s = fmaf(s, d, 1.0f / 24.0f);
+      s = fmaf(s, d, 1.0f / 6.0f);
+      s = fmaf(s, d, 0.5f);
+      p.kl = s * d * d;
+    } else {
+      p.kl = expf(d) - d - 1.0f;
+    }
+    p.value = fmaf(c.kl_coef, p.kl, p.value);
+    p.slope = fmaf(-c.kl_coef, d + p.kl, p.slope);
+  }
+  return p;
+}
+
+}  // namespace b2

@@ -395,6 +395,26 @@ def ref_policy(lp, old, adv, ref, mask, low, high, kl_coef):
     return (w * value).sum() / total, (w * kl).sum() / total, (w * cut).sum() / total
 
 
+def policy_tol(lp, old, adv, ref, mask, kl_coef):
+    """How far a token's term and slope may be off, computed in 32 bits: the ratio by its exponent's rounding
+    (u |lp - old|), expf's ulp (2u) and one product; exp(d) - d - 1 by d's rounding, whose relative effect is at most
+    2 + |d| times u |d| / |d|, ten roundings of its series (each below u of the result) or of the subtraction at |d| > 1
+    (4u); one fused multiply-add.  -> (sum of the terms' errors / total weight, slopes' errors / total weight)"""
+    w = torch.ones(lp.shape, dtype=torch.float64) if mask is None else mask.double()
+    keep = w != 0
+    lp, old, adv = (torch.where(keep, a.double(), torch.zeros_like(w)) for a in (lp, old, adv))
+    ra = (torch.exp(lp - old) * adv).abs()
+    value = U * ((lp - old).abs() + 6) * ra
+    slope = value.clone()
+    if ref is not None:
+        d = torch.where(keep, ref.double(), torch.zeros_like(w)) - lp
+        kl = torch.expm1(d) - d
+        value = value + kl_coef * U * (2 + d.abs() + 12) * kl
+        slope = slope + kl_coef * U * ((2 + d.abs() + 12) * kl + 3 * d.abs() + 2 * torch.expm1(d).abs())
+    total = max(float(w.sum()), 1e-300)
+    return float((w.abs() * value).sum() / total), 2 * w.abs() * slope / total
+
+
 POLICY = [(1, None, True, 0.0), (64, "bool", True, 0.05), (4097, "float", True, 0.02), (333, "uint8", False, 0.0),
           (1000003, "bool", True, 0.1), (50, "none counts", True, 0.1)]
 
@@ -422,11 +442,12 @@ def test_policy_loss(otf, n, mask, has_ref, kl):
     leaf = lp.cuda().requires_grad_()
     cuda = [None if a is None else a.cuda() for a in (old, adv, ref, w)]
     got = otf.losses.policy_loss(leaf, *cuda, clip_low=0.2, clip_high=0.28, kl_coef=kl)
-    # 64-bit arithmetic: the store's half step, and what cancels in a sum of n terms of order 1 in 64 bits
-    for a, b in zip(got, (loss, mean_kl, share)):
-        close(a.detach().cpu(), b.detach(), 2 * U * b.detach().abs() + 1e-12)
+    # the terms' errors, added in 64 bits, and the store's half step
+    off, slope_off = policy_tol(lp, old, adv, ref, w, kl)
+    for a, b, o in zip(got, (loss, mean_kl, share), (off, off / kl if kl else 0.0, 0.0)):
+        close(a.detach().cpu(), b.detach(), o + 2 * U * b.detach().abs() + 1e-12)
     grad, = torch.autograd.grad(got[0], leaf, torch.tensor(3.0, device="cuda"))
-    close(grad.cpu(), 3 * want, 4 * U * 3 * want.abs() + 1e-12 * want.abs().max(), "gradient")
+    close(grad.cpu(), 3 * want, 3 * slope_off + 6 * U * 3 * want.abs(), "gradient")
 
 
 def test_policy_borders(otf):
@@ -476,22 +497,25 @@ def test_policy_loss_with_grad(otf, rows, classes, dtype):
     _, rel_s, _ = parts(counted)
     lp_tol = float((rel_s[:, 0] + 2 * U * exact.abs() + U).max())
     slope = float(adv.abs().max()) * 1.5 + 0.1  # how fast a token's loss moves with its log-probability
-    for a, b in zip(got[:2], (loss, kl)):
-        close(a.cpu(), b.detach(), slope * lp_tol + 2 * U * b.detach().abs())
+    term_off, slope_off = policy_tol(exact.cpu(), old, adv, ref, w, 0.04)
+    loss_off = slope * lp_tol + term_off + 2 * U * float(loss.detach().abs())
+    kl_off = lp_tol + term_off / 0.04 + 2 * U * float(kl.detach().abs())
+    for a, b, o in zip(got[:2], (loss, kl), (loss_off, kl_off)):
+        close(a.cpu(), b.detach(), o)
     close(got[2].cpu(), share, 2 * U * share)
     want, tol = ref_log_probs_grad(counted, t, 32 * up * keep, x.dtype)
     p = parts(counted)[0]
     onehot = torch.zeros_like(p).scatter_(1, t.clamp(0, classes - 1)[:, None], 1.0)
-    moved = (32 * lp_tol * slope / max(1, int(w.sum())) * (valid & keep))[:, None] * (p - onehot).abs()
+    moved = (32 * (lp_tol * slope / max(1, int(w.sum())) + slope_off.cuda()) * (valid & keep))[:, None] * (p - onehot).abs()
     close(got[3], want, tol + moved, "gradient")
     # the same as its parts, one after the other
     leaf = counted.clone().requires_grad_()
     whole = otf.losses.policy_loss(otf.losses.token_log_probs(leaf, t), old.cuda(), adv.cuda(), ref.cuda(), w.cuda(),
                                    clip_low=0.2, clip_high=0.28, kl_coef=0.04)
-    for a, b in zip(got[:3], whole):
-        close(a, b.detach(), 2 * U * b.detach().abs() + 1e-12)
+    for a, b, o in zip(got[:3], whole, (2 * loss_off, 2 * kl_off, 0.0)):  # each is that near to the definition
+        close(a, b.detach(), o + 4 * U * b.detach().abs())
     d, = torch.autograd.grad(whole[0], leaf, gl)
-    close(got[3], d, 8 * U * d.abs().double() + 2 * torch.finfo(x.dtype).eps * d.abs().double() + 2 * TINY[x.dtype])
+    close(got[3], d, 2 * (tol + moved), "gradient by parts")
 
 
 # ---------------------------------------------------------------- together
