@@ -431,7 +431,9 @@ int b2_token_log_probs_grad(b2_stream_t stream, const b2_logits_t* logits,
  * With grad_logits, the gradient too, in the same pass over the scores:
  *   grad[r, j] = grad_loss * temperature * w[r] / sum w
  *                * (P[r, j] - sum_{k: id[r,k] == j} q[r,k])
- * grad_loss: a device float, or null for 1.  row_stats as above or null. */
+ * grad_loss: a device float, or null for 1.  row_stats: 4 * rows + 2 floats,
+ * 8-byte aligned, for b2_distillation_loss_grad (each row's statistics as above,
+ * the sum of the weights and room for the rows' losses), or null. */
 int b2_distillation_loss(b2_stream_t stream, const b2_logits_t* logits,
                          const void* teacher_ids, int id_bytes,
                          const void* teacher_logits, int teacher_dtype,

@@ -65,20 +65,26 @@ __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
   if (blockIdx.x == 0 && threadIdx.x == 0) *total = v[0];
 }
 
-// *loss and stats[k - 1] = sum_r values[k][r] / total, 0 when the total is 0.
+// *loss and stats[k - 1] = sum_r values[k][r] / total, 0 when the total is 0.  The total is
+// *total_in, or the sum of the weights (rows without any); total_out: null, or where it goes.
 template <int kN>
 __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
-    mean_kernel(const double* __restrict__ values, const double* __restrict__ total, int64_t rows,
+    mean_kernel(const double* __restrict__ values, const void* __restrict__ weights, int weight_bytes,
+                const double* __restrict__ total_in, double* __restrict__ total_out, int64_t rows,
                 float* __restrict__ loss, float* __restrict__ stats) {
-  double v[kN] = {};
-  for (int64_t i = (int64_t)blockIdx.x * kSumThreads + threadIdx.x; i < rows; i += kSumCtas * kSumThreads)
+  const bool add = total_in == nullptr && weights != nullptr;
+  double v[kN + 1] = {};
+  for (int64_t i = (int64_t)blockIdx.x * kSumThreads + threadIdx.x; i < rows; i += kSumCtas * kSumThreads) {
 #pragma unroll
     for (int k = 0; k < kN; ++k) v[k] += values[k * rows + i];
-  cluster_sum<kN>(v);
+    if (add) v[kN] += (double)weight_at(weights, weight_bytes, i);
+  }
+  cluster_sum<kN + 1>(v);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    const double t = total != nullptr ? *total : (double)rows;
+    const double t = total_in != nullptr ? *total_in : add ? v[kN] : (double)rows;
 #pragma unroll
     for (int k = 0; k < kN; ++k) (k == 0 ? loss : stats + k - 1)[0] = t != 0.0 ? (float)(v[k] / t) : 0.0f;
+    if (total_out != nullptr) *total_out = t;
   }
 }
 
@@ -102,18 +108,23 @@ struct PreferenceArgs {
   double beta, smoothing;
 };
 
+// The sum of a sequence's w (lp - ref) by `threads` threads, t among them.
+__device__ __forceinline__ double sequence_part(const PreferenceArgs& A, int64_t i, int t, int threads) {
+  const int64_t a = offset_at(A.offsets, A.offset_bytes, i, A.tokens);
+  const int64_t b = offset_at(A.offsets, A.offset_bytes, i + 1, A.tokens);
+  double v = 0.0;
+  for (int64_t n = a + t; n < b; n += threads) {
+    const float w = weight_at(A.mask, A.mask_bytes, n);
+    if (w != 0.0f) v += (double)w * ((double)A.lp[n] - (A.ref != nullptr ? (double)A.ref[n] : 0.0));
+  }
+  return v;
+}
+
 // One CTA per sequence: rewards[i] = beta sum_n w_n (lp_n - ref_n).
 __global__ void __launch_bounds__(kTokenThreads) sequence_sum_kernel(const PreferenceArgs A, double* __restrict__ sums) {
   __shared__ double part[kTokenThreads / 32];
   const int64_t i = blockIdx.x;
-  const int64_t a = offset_at(A.offsets, A.offset_bytes, i, A.tokens);
-  const int64_t b = offset_at(A.offsets, A.offset_bytes, i + 1, A.tokens);
-  double v = 0.0;
-  for (int64_t n = a + threadIdx.x; n < b; n += kTokenThreads) {
-    const float w = weight_at(A.mask, A.mask_bytes, n);
-    if (w != 0.0f) v += (double)w * ((double)A.lp[n] - (A.ref != nullptr ? (double)A.ref[n] : 0.0));
-  }
-  v = warp_sum(v);
+  const double v = warp_sum(sequence_part(A, i, threadIdx.x, kTokenThreads));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -125,22 +136,53 @@ __global__ void __launch_bounds__(kTokenThreads) sequence_sum_kernel(const Prefe
 
 __device__ __forceinline__ double softplus(double z) { return fmax(z, 0.0) + log1p(exp(-fabs(z))); }
 
+// One pair's loss; its rewards and its sequences' slopes are written.
+__device__ __forceinline__ double pair_loss(const PreferenceArgs& A, int64_t p, double chosen, double rejected,
+                                            float* __restrict__ rewards, float* __restrict__ slopes) {
+  const double eps = A.smoothing, h = chosen - rejected;
+  // sigma(h) and sigma(-h), each without cancellation
+  const double z = exp(-fabs(h)), small = z / (1.0 + z), large = 1.0 / (1.0 + z);
+  const double up = h >= 0.0 ? large : small, down = h >= 0.0 ? small : large;
+  const double slope = (eps * up - (1.0 - eps) * down) * A.beta / (double)A.pairs;
+  rewards[p] = (float)chosen;
+  rewards[A.pairs + p] = (float)rejected;
+  slopes[p] = (float)slope;
+  slopes[A.pairs + p] = (float)-slope;
+  return (1.0 - eps) * softplus(-h) + eps * softplus(h);
+}
+
 __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
     pair_kernel(const PreferenceArgs A, const double* __restrict__ sums, float* __restrict__ loss,
                 float* __restrict__ rewards, float* __restrict__ slopes) {
   double v[1] = {0.0};
-  const double eps = A.smoothing;
-  for (int64_t p = (int64_t)blockIdx.x * kSumThreads + threadIdx.x; p < A.pairs; p += kSumCtas * kSumThreads) {
-    const double chosen = sums[p], rejected = sums[A.pairs + p], h = chosen - rejected;
-    v[0] += (1.0 - eps) * softplus(-h) + eps * softplus(h);
-    // sigma(h) and sigma(-h), each without cancellation
-    const double z = exp(-fabs(h)), small = z / (1.0 + z), large = 1.0 / (1.0 + z);
-    const double up = h >= 0.0 ? large : small, down = h >= 0.0 ? small : large;
-    const double slope = (eps * up - (1.0 - eps) * down) * A.beta / (double)A.pairs;
-    rewards[p] = (float)chosen;
-    rewards[A.pairs + p] = (float)rejected;
-    slopes[p] = (float)slope;
-    slopes[A.pairs + p] = (float)-slope;
+  for (int64_t p = (int64_t)blockIdx.x * kSumThreads + threadIdx.x; p < A.pairs; p += kSumCtas * kSumThreads)
+    v[0] += pair_loss(A, p, sums[p], sums[A.pairs + p], rewards, slopes);
+  cluster_sum<1>(v);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *loss = (float)(v[0] / (double)A.pairs);
+}
+
+// A few pairs of short sequences in one launch: each CTA of the cluster takes
+// pairs in turn, half of its warps a sequence.
+constexpr int kFewPairs = 4 * kSumCtas;
+constexpr int kFewTokens = 32768;
+
+__global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
+    few_pairs_kernel(const PreferenceArgs A, float* __restrict__ loss, float* __restrict__ rewards,
+                     float* __restrict__ slopes) {
+  constexpr int kHalf = kSumThreads / 2, kWarps = kSumThreads / 32;
+  __shared__ double part[2][kWarps];
+  double v[1] = {0.0};
+  int turn = 0;
+  for (int64_t p = blockIdx.x; p < A.pairs; p += kSumCtas, turn ^= 1) {
+    const int half = threadIdx.x / kHalf;
+    const double sum = warp_sum(sequence_part(A, p + half * A.pairs, threadIdx.x % kHalf, kHalf));
+    if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double chosen = 0.0, rejected = 0.0;
+      for (int k = 0; k < kWarps / 2; ++k) chosen += part[turn][k], rejected += part[turn][kWarps / 2 + k];
+      v[0] += pair_loss(A, p, A.beta * chosen, A.beta * rejected, rewards, slopes);
+    }
   }
   cluster_sum<1>(v);
   if (blockIdx.x == 0 && threadIdx.x == 0) *loss = (float)(v[0] / (double)A.pairs);
@@ -180,16 +222,14 @@ struct PolicyArgs {
 
 constexpr int kPolicySums = 4;  // loss, kl, clipped, weights
 
-__global__ void __launch_bounds__(kTokenThreads)
-    policy_kernel(const PolicyArgs A, float* __restrict__ slopes, double* __restrict__ partial) {
-  __shared__ double part[kPolicySums][kTokenThreads / 32];
-  double v[kPolicySums] = {};
-  for (int64_t n = (int64_t)blockIdx.x * kTokenThreads + threadIdx.x; n < A.tokens;
-       n += (int64_t)gridDim.x * kTokenThreads) {
+// What thread `first` of every `step` adds up (loss, kl, clipped, weights); the tokens' slopes are written.
+__device__ __forceinline__ void policy_part(const PolicyArgs& A, int64_t first, int64_t step, float* __restrict__ slopes,
+                                            double* v) {
+  const bool has_ref = A.ref_lp != nullptr;
+  for (int64_t n = first; n < A.tokens; n += step) {
     const float w = weight_at(A.mask, A.mask_bytes, n);
     float slope = 0.0f;
     if (w != 0.0f) {
-      const bool has_ref = A.ref_lp != nullptr;
       const PolicyTerm t =
           policy_term(A.lp[n], PolicyToken{A.old_lp[n], A.advantages[n], has_ref ? A.ref_lp[n] : 0.0f, has_ref}, A.clip);
       slope = w * t.slope;
@@ -200,6 +240,33 @@ __global__ void __launch_bounds__(kTokenThreads)
     }
     if (slopes != nullptr) slopes[n] = slope;
   }
+}
+
+// *loss, stats = {mean KL, clipped share, 1 / sum of the weights}, all 0 when the weights sum to 0.
+__device__ __forceinline__ void store_means(const double* v, float* __restrict__ loss, float* __restrict__ stats) {
+  const double inv = v[3] != 0.0 ? 1.0 / v[3] : 0.0;
+  *loss = v[3] != 0.0 ? (float)(v[0] / v[3]) : 0.0f;
+  stats[0] = v[3] != 0.0 ? (float)(v[1] / v[3]) : 0.0f;
+  stats[1] = v[3] != 0.0 ? (float)(v[2] / v[3]) : 0.0f;
+  stats[2] = (float)inv;
+}
+
+// Few tokens in one launch, by one cluster.
+constexpr int kFewPolicyTokens = 8 * kSumCtas * kSumThreads;
+
+__global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
+    few_policy_kernel(const PolicyArgs A, float* __restrict__ slopes, float* __restrict__ loss, float* __restrict__ stats) {
+  double v[kPolicySums] = {};
+  policy_part(A, (int64_t)blockIdx.x * kSumThreads + threadIdx.x, kSumCtas * kSumThreads, slopes, v);
+  cluster_sum<kPolicySums>(v);
+  if (blockIdx.x == 0 && threadIdx.x == 0) store_means(v, loss, stats);
+}
+
+__global__ void __launch_bounds__(kTokenThreads)
+    policy_kernel(const PolicyArgs A, float* __restrict__ slopes, double* __restrict__ partial) {
+  __shared__ double part[kPolicySums][kTokenThreads / 32];
+  double v[kPolicySums] = {};
+  policy_part(A, (int64_t)blockIdx.x * kTokenThreads + threadIdx.x, (int64_t)gridDim.x * kTokenThreads, slopes, v);
 #pragma unroll
   for (int k = 0; k < kPolicySums; ++k) {
     v[k] = warp_sum(v[k]);
@@ -213,7 +280,6 @@ __global__ void __launch_bounds__(kTokenThreads)
   }
 }
 
-// *loss, stats = {mean KL, clipped share, 1 / sum of the weights}, all 0 when the weights sum to 0.
 __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
     policy_mean_kernel(const double* __restrict__ partial, int64_t parts, float* __restrict__ loss,
                        float* __restrict__ stats) {
@@ -222,13 +288,7 @@ __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
 #pragma unroll
     for (int k = 0; k < kPolicySums; ++k) v[k] += partial[k * parts + i];
   cluster_sum<kPolicySums>(v);
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    const double inv = v[3] != 0.0 ? 1.0 / v[3] : 0.0;
-    *loss = v[3] != 0.0 ? (float)(v[0] / v[3]) : 0.0f;
-    stats[0] = v[3] != 0.0 ? (float)(v[1] / v[3]) : 0.0f;
-    stats[1] = v[3] != 0.0 ? (float)(v[2] / v[3]) : 0.0f;
-    stats[2] = (float)inv;
-  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) store_means(v, loss, stats);
 }
 
 __global__ void __launch_bounds__(kTokenThreads)
@@ -365,22 +425,28 @@ int b2_distillation_loss(b2_stream_t stream, const b2_logits_t* logits, const vo
   B2_RETURN_IF_ERROR(distill_args(logits, teacher_ids, id_bytes, teacher_logits, teacher_dtype, top, weights,
                                   weight_bytes, temperature, "distillation_loss", &a));
   B2_REQUIRE(loss != nullptr, "distillation_loss: null pointer");
+  B2_REQUIRE((reinterpret_cast<uintptr_t>(row_stats) & 7) == 0, "distillation_loss: row_stats must be 8-byte aligned");
   const DeviceInfo* d = nullptr;
   B2_RETURN_IF_ERROR(device_info(&d));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // row_stats: statistics [rows][2], the sum of the weights (64 bits), the rows' losses (64 bits)
   Scratch scratch;
-  B2_RETURN_IF_ERROR(scratch.alloc((a.rows + 1) * sizeof(double), s));
-  double* total = weights != nullptr ? scratch.as<double>() + a.rows : nullptr;
-  if (total != nullptr)
-    B2_RETURN_IF_ERROR(sum_weights(s, weights, weight_bytes, a.rows, total, "distillation_loss"));
-  a.total = total;
-  a.row_out = scratch.as<double>();
+  double* total = reinterpret_cast<double*>(row_stats + 2 * a.rows);
+  if (row_stats == nullptr) {
+    B2_RETURN_IF_ERROR(scratch.alloc((a.rows + 1) * sizeof(double), s));
+    total = scratch.as<double>();
+  }
+  a.row_out = total + 1;
+  const bool early = grad_logits != nullptr && weights != nullptr;  // the gradient divides by the sum
+  if (early) B2_RETURN_IF_ERROR(sum_weights(s, weights, weight_bytes, a.rows, total, "distillation_loss"));
+  a.total = early ? total : nullptr;
   a.stats = reinterpret_cast<float2*>(row_stats);
   a.grad_loss = grad_loss;
   a.grad = grad_logits;
   B2_RETURN_IF_ERROR(
       launch_rows(s, a, logits->dtype, kDistill, true, grad_logits != nullptr, d, "distillation_loss"));
-  mean_kernel<1><<<kSumCtas, kSumThreads, 0, s>>>(a.row_out, total, a.rows, loss, nullptr);
+  mean_kernel<1><<<kSumCtas, kSumThreads, 0, s>>>(a.row_out, weights, weight_bytes, a.total, total, a.rows, loss,
+                                                  nullptr);
   return check_launch(s, "distillation_loss");
 }
 
@@ -397,13 +463,7 @@ int b2_distillation_loss_grad(b2_stream_t stream, const b2_logits_t* logits, con
   const DeviceInfo* d = nullptr;
   B2_RETURN_IF_ERROR(device_info(&d));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  Scratch scratch;
-  if (weights != nullptr) {
-    B2_RETURN_IF_ERROR(scratch.alloc(sizeof(double), s));
-    B2_RETURN_IF_ERROR(
-        sum_weights(s, weights, weight_bytes, a.rows, scratch.as<double>(), "distillation_loss_grad"));
-    a.total = scratch.as<double>();
-  }
+  a.total = reinterpret_cast<const double*>(row_stats + 2 * a.rows);
   a.stats = reinterpret_cast<float2*>(const_cast<float*>(row_stats));
   a.grad_loss = grad_loss;
   a.grad = grad_logits;
@@ -429,6 +489,10 @@ int b2_preference_loss(b2_stream_t stream, const float* log_probs, const float* 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const PreferenceArgs a{log_probs, ref_log_probs, mask, mask_bytes, tokens, offsets, offset_bytes, pairs, beta,
                          label_smoothing};
+  if (pairs <= kFewPairs && tokens <= kFewTokens) {
+    few_pairs_kernel<<<kSumCtas, kSumThreads, 0, s>>>(a, loss, rewards, slopes);
+    return check_launch(s, what);
+  }
   Scratch scratch;
   B2_RETURN_IF_ERROR(scratch.alloc(2 * pairs * sizeof(double), s));
   sequence_sum_kernel<<<(unsigned)(2 * pairs), kTokenThreads, 0, s>>>(a, scratch.as<double>());
@@ -479,6 +543,10 @@ int b2_policy_loss(b2_stream_t stream, const float* log_probs, const float* old_
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const PolicyArgs a{log_probs, old_log_probs, ref_log_probs, advantages, mask, mask_bytes, tokens,
                      PolicyClip{1.0 - clip_low, 1.0 + clip_high, (float)kl_coef}};
+  if (tokens <= kFewPolicyTokens) {
+    few_policy_kernel<<<kSumCtas, kSumThreads, 0, s>>>(a, slopes, loss, stats);
+    return check_launch(s, what);
+  }
   const int grid = grid_for(tokens, kTokenThreads, 4);
   Scratch scratch;
   B2_RETURN_IF_ERROR(scratch.alloc((size_t)grid * kPolicySums * sizeof(double), s));
@@ -535,7 +603,7 @@ int b2_policy_loss_with_grad(b2_stream_t stream, const b2_logits_t* logits, cons
   a.row_out = scratch.as<double>();
   a.grad = grad_logits;
   B2_RETURN_IF_ERROR(launch_rows(s, a, logits->dtype, kPolicy, true, true, d, what));
-  mean_kernel<3><<<kSumCtas, kSumThreads, 0, s>>>(a.row_out, total, a.rows, loss, stats);
+  mean_kernel<3><<<kSumCtas, kSumThreads, 0, s>>>(a.row_out, nullptr, 0, total, nullptr, a.rows, loss, stats);
   return check_launch(s, what);
 }
 

@@ -596,8 +596,15 @@ def _k_upsampling_bilinear2d_grad(grad_out, input_sizes, size):
 
 
 # ------------------------------------------- losses over rows of class scores
+#
+# A call's cost on the host counts here (a few tokens' losses take the GPU
+# microseconds): arguments are checked in one test each, with the reason looked for
+# only when it fails, and the stream is fetched as a plain handle.
 
 _FLOATS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # b2_dtype_t
+_INTS = (torch.int64, torch.int32)
+_WEIGHTS = (torch.float32, torch.bool, torch.uint8)
+_F32_ONLY = (torch.float32,)
 
 
 def _on_cuda(t, what: str) -> None:
@@ -612,7 +619,8 @@ def _logits(t, what: str):
     """(tensor, b2_logits_t) of scores [..., classes]; leading axes that fold
     into two strides are read in place, others are copied."""
     _on_cuda(t, what)
-    if t.dtype not in _FLOATS:
+    dtype = _FLOATS.get(t.dtype)
+    if dtype is None:
         raise errors.InvalidArgumentError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
     if t.dim() < 1 or t.shape[-1] < 1:
         raise errors.InvalidArgumentError(f"{what} must be [..., classes] with at least one class")
@@ -628,44 +636,37 @@ def _logits(t, what: str):
                 axes.append((size, stride))
         if len(axes) <= 2 and (t.stride(-1) == 1 or classes == 1):
             (outer, so), (inner, si) = [(1, 0)] * (2 - len(axes)) + axes
-            return t, Logits(t.data_ptr(), _FLOATS[t.dtype], outer, inner, classes, so, si)
+            return t, Logits(t.data_ptr(), dtype, outer, inner, classes, so, si)
         t = t.contiguous()
-    return t, Logits(t.data_ptr(), _FLOATS[t.dtype], 1, t.numel() // classes, classes, 0, classes)
+    return t, Logits(t.data_ptr(), dtype, 1, t.numel() // classes, classes, 0, classes)
 
 
-def _same(t, what: str, shape, device, dtypes, names: str) -> torch.Tensor:
+def _refuse(t, what, shape, dev, dtypes):
     _on_cuda(t, what)
     if t.dtype not in dtypes:
+        names = ", ".join(str(d).removeprefix("torch.") for d in dtypes)
         raise errors.InvalidArgumentError(f"{what} must be {names}, got {t.dtype}")
     if t.shape != shape:
         raise errors.InvalidArgumentError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != device:
-        raise errors.InvalidArgumentError(f"{what} must live on {device}, got {t.device}")
+    raise errors.InvalidArgumentError(f"{what} must live on cuda:{dev}, got {t.device}")
+
+
+def _same(t, what: str, shape, dev: int, dtypes) -> torch.Tensor:
+    if not (isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype in dtypes and t.shape == shape):
+        _refuse(t, what, shape, dev, dtypes)
     return t if t.is_contiguous() else t.contiguous()
 
 
-_INTS = (torch.int64, torch.int32)
-_WEIGHTS = (torch.float32, torch.bool, torch.uint8)
+def _opt_same(t, what, shape, dev, dtypes):
+    return None if t is None else _same(t, what, shape, dev, dtypes)
 
 
-def _ints(t, what, shape, device):
-    return _same(t, what, shape, device, _INTS, "int32 or int64")
-
-
-def _per_token(t, what, shape, device):
-    return None if t is None else _same(t, what, shape, device, (torch.float32,), "float32")
-
-
-def _weights(t, what, shape, device):
-    return None if t is None else _same(t, what, shape, device, _WEIGHTS, "float32, bool or uint8")
-
-
-def _scalar(t, what, device):
+def _scalar(t, what, dev):
     if t is None:
         return None
-    _on_cuda(t, what)
-    if t.dtype != torch.float32 or t.numel() != 1 or t.device != device:
-        raise errors.InvalidArgumentError(f"{what} must be a float32 scalar on {device}")
+    if not (isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype == torch.float32 and t.numel() == 1):
+        _on_cuda(t, what)
+        raise errors.InvalidArgumentError(f"{what} must be a float32 scalar on cuda:{dev}")
     return t
 
 
@@ -677,137 +678,142 @@ def _size(t):
     return 0 if t is None else t.element_size()
 
 
-def _f32(shape, device):
-    return torch.empty(shape, device=device, dtype=torch.float32)
+def _f32(like, shape):
+    return like.new_empty(shape, dtype=torch.float32)
 
 
-def _dense_like(x):
-    return torch.empty(x.shape, device=x.device, dtype=x.dtype)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call(dev: int, entry, *args) -> None:
+    """Calls a C entry on device ``dev`` and torch's current stream of it."""
+    if torch.cuda.current_device() == dev:
+        rc = entry(_raw_stream(dev), *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(_raw_stream(dev), *args)
+    if rc:
+        _check(rc)
 
 
 def _k_token_log_probs(logits, targets, with_stats=False):
     x, v = _logits(logits, "logits")
-    t = _ints(targets, "targets", x.shape[:-1], x.device)
-    out = _f32(t.shape, x.device)
-    stats = _f32((*t.shape, 2), x.device) if with_stats else None
-    with _on_device(x):
-        _check(_lib.b2_token_log_probs(_stream(x), ctypes.byref(v), _p(t), t.element_size(), _p(out), _opt(stats)))
+    dev, lead = x.get_device(), x.shape[:-1]
+    t = _same(targets, "targets", lead, dev, _INTS)
+    out = _f32(x, lead)
+    stats = _f32(x, (*lead, 2)) if with_stats else None
+    _call(dev, _lib.b2_token_log_probs, ctypes.byref(v), t.data_ptr(), t.element_size(), out.data_ptr(), _opt(stats))
     return (out, stats) if with_stats else out
 
 
 def _k_token_log_probs_grad(grad_log_probs, logits, targets, row_stats):
     x, v = _logits(logits, "logits")
-    t = _ints(targets, "targets", x.shape[:-1], x.device)
-    g = _per_token(grad_log_probs, "grad_log_probs", t.shape, x.device)
-    st = _per_token(row_stats, "row_stats", (*t.shape, 2), x.device)
-    if g is None or st is None:
-        raise errors.InvalidArgumentError("grad_log_probs and row_stats must be torch tensors on a CUDA device")
-    out = _dense_like(x)
-    with _on_device(x):
-        _check(_lib.b2_token_log_probs_grad(_stream(x), ctypes.byref(v), _p(t), t.element_size(), _p(st), _p(g),
-                                            _p(out)))
+    dev, lead = x.get_device(), x.shape[:-1]
+    t = _same(targets, "targets", lead, dev, _INTS)
+    g = _same(grad_log_probs, "grad_log_probs", lead, dev, _F32_ONLY)
+    out = x.new_empty(x.shape)
+    _call(dev, _lib.b2_token_log_probs_grad, ctypes.byref(v), t.data_ptr(), t.element_size(), row_stats.data_ptr(),
+          g.data_ptr(), out.data_ptr())
     return out
 
 
-def _teacher(x, teacher_ids, teacher_logits, weights):
-    lead = x.shape[:-1]
+def _teacher(x, dev, lead, teacher_ids, teacher_logits, weights):
     if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dim() != x.dim():
         raise errors.InvalidArgumentError("teacher_ids must be [..., entries] with the leading axes of logits")
-    ids = _ints(teacher_ids, "teacher_ids", (*lead, teacher_ids.shape[-1]), x.device)
-    y = _same(teacher_logits, "teacher_logits", ids.shape, x.device, _FLOATS, "float32, float16 or bfloat16")
-    return ids, y, _weights(weights, "weights", lead, x.device)
+    ids = _same(teacher_ids, "teacher_ids", (*lead, teacher_ids.shape[-1]), dev, _INTS)
+    y = _same(teacher_logits, "teacher_logits", ids.shape, dev, _FLOATS)
+    return ids, y, _opt_same(weights, "weights", lead, dev, _WEIGHTS)
 
 
 def _k_distillation_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0, with_stats=False,
                          with_grad=False, grad_loss=None):
     x, v = _logits(logits, "logits")
-    ids, y, w = _teacher(x, teacher_ids, teacher_logits, weights)
-    gl = _scalar(grad_loss, "grad_loss", x.device)
-    loss = _f32((), x.device)
-    stats = _f32((*x.shape[:-1], 2), x.device) if with_stats else None
-    grad = _dense_like(x) if with_grad else None
-    with _on_device(x):
-        _check(_lib.b2_distillation_loss(_stream(x), ctypes.byref(v), _p(ids), ids.element_size(), _p(y),
-                                         _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w), float(temperature),
-                                         _p(loss), _opt(stats), _opt(gl), _opt(grad)))
+    dev, lead = x.get_device(), x.shape[:-1]
+    ids, y, w = _teacher(x, dev, lead, teacher_ids, teacher_logits, weights)
+    gl = _scalar(grad_loss, "grad_loss", dev)
+    loss = _f32(x, ())
+    stats = _f32(x, 4 * (v.outer * v.inner) + 2) if with_stats else None
+    grad = x.new_empty(x.shape) if with_grad else None
+    _call(dev, _lib.b2_distillation_loss, ctypes.byref(v), ids.data_ptr(), ids.element_size(), y.data_ptr(),
+          _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w), float(temperature), loss.data_ptr(), _opt(stats),
+          _opt(gl), _opt(grad))
     return (loss, stats) if with_stats else (loss, grad) if with_grad else loss
 
 
 def _k_distillation_loss_grad(logits, teacher_ids, teacher_logits, weights, temperature, row_stats, grad_loss):
     x, v = _logits(logits, "logits")
-    ids, y, w = _teacher(x, teacher_ids, teacher_logits, weights)
-    gl = _scalar(grad_loss, "grad_loss", x.device)
-    st = _per_token(row_stats, "row_stats", (*x.shape[:-1], 2), x.device)
-    if gl is None or st is None:
-        raise errors.InvalidArgumentError("grad_loss and row_stats must be torch tensors on a CUDA device")
-    out = _dense_like(x)
-    with _on_device(x):
-        _check(_lib.b2_distillation_loss_grad(_stream(x), ctypes.byref(v), _p(ids), ids.element_size(), _p(y),
-                                              _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w),
-                                              float(temperature), _p(st), _p(gl), _p(out)))
+    dev, lead = x.get_device(), x.shape[:-1]
+    ids, y, w = _teacher(x, dev, lead, teacher_ids, teacher_logits, weights)
+    gl = _scalar(grad_loss, "grad_loss", dev)
+    out = x.new_empty(x.shape)
+    _call(dev, _lib.b2_distillation_loss_grad, ctypes.byref(v), ids.data_ptr(), ids.element_size(), y.data_ptr(),
+          _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w), float(temperature), row_stats.data_ptr(),
+          gl.data_ptr(), out.data_ptr())
     return out
 
 
-def _offsets(offsets, device):
-    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 3 or offsets.numel() % 2 == 0:
-        raise errors.InvalidArgumentError("offsets must have 2 * pairs + 1 elements, pairs >= 1")
-    return _ints(offsets, "offsets", offsets.shape, device), offsets.numel() // 2
+def _log_probs(t, what="log_probs"):
+    _on_cuda(t, what)
+    if t.dtype != torch.float32:
+        raise errors.InvalidArgumentError(f"{what} must be float32, got {t.dtype}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _k_preference_loss(log_probs, offsets, ref_log_probs=None, mask=None, beta=0.1, label_smoothing=0.0):
     """-> loss, rewards [2 * pairs], slopes [2 * pairs]"""
-    lp = _input(log_probs, "log_probs")
-    off, pairs = _offsets(offsets, lp.device)
-    ref = _per_token(ref_log_probs, "ref_log_probs", lp.shape, lp.device)
-    w = _weights(mask, "mask", lp.shape, lp.device)
-    loss, rewards, slopes = _f32((), lp.device), _f32(2 * pairs, lp.device), _f32(2 * pairs, lp.device)
-    with _on_device(lp):
-        _check(_lib.b2_preference_loss(_stream(lp), _p(lp), _opt(ref), _opt(w), _size(w), lp.numel(), _p(off),
-                                       off.element_size(), pairs, float(beta), float(label_smoothing), _p(loss),
-                                       _p(rewards), _p(slopes)))
+    lp = _log_probs(log_probs)
+    dev, shape = lp.get_device(), lp.shape
+    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 3 or offsets.numel() % 2 == 0:
+        raise errors.InvalidArgumentError("offsets must have 2 * pairs + 1 elements, pairs >= 1")
+    off = _same(offsets, "offsets", offsets.shape, dev, _INTS)
+    ref = _opt_same(ref_log_probs, "ref_log_probs", shape, dev, _F32_ONLY)
+    w = _opt_same(mask, "mask", shape, dev, _WEIGHTS)
+    sequences = off.numel() - 1
+    loss, rewards, slopes = lp.new_empty(()), lp.new_empty(sequences), lp.new_empty(sequences)
+    _call(dev, _lib.b2_preference_loss, lp.data_ptr(), _opt(ref), _opt(w), _size(w), lp.numel(), off.data_ptr(),
+          off.element_size(), sequences // 2, float(beta), float(label_smoothing), loss.data_ptr(),
+          rewards.data_ptr(), slopes.data_ptr())
     return loss, rewards, slopes
 
 
 def _k_preference_loss_grad(grad_loss, slopes, offsets, mask, shape):
-    device = slopes.device
-    gl = _scalar(grad_loss, "grad_loss", device)
-    off, pairs = _offsets(offsets, device)
-    sl = _per_token(slopes, "slopes", (2 * pairs,), device)
-    w = _weights(mask, "mask", shape, device)
-    out = _f32(shape, device)
-    with _on_device(out):
-        _check(_lib.b2_preference_loss_grad(_stream(out), _p(gl), _p(sl), _opt(w), _size(w), out.numel(), _p(off),
-                                            off.element_size(), pairs, _p(out)))
+    dev = slopes.get_device()
+    gl = _scalar(grad_loss, "grad_loss", dev)
+    off = offsets if offsets.is_contiguous() else offsets.contiguous()
+    w = _opt_same(mask, "mask", shape, dev, _WEIGHTS)
+    out = slopes.new_empty(shape)
+    _call(dev, _lib.b2_preference_loss_grad, gl.data_ptr(), slopes.data_ptr(), _opt(w), _size(w), out.numel(),
+          off.data_ptr(), off.element_size(), slopes.numel() // 2, out.data_ptr())
     return out
 
 
-def _policy_inputs(shape, device, old_log_probs, advantages, ref_log_probs, mask):
-    old = _per_token(old_log_probs, "old_log_probs", shape, device)
-    adv = _per_token(advantages, "advantages", shape, device)
-    if old is None or adv is None:
-        raise errors.InvalidArgumentError("old_log_probs and advantages must be torch tensors on a CUDA device")
-    return old, adv, _per_token(ref_log_probs, "ref_log_probs", shape, device), _weights(mask, "mask", shape, device)
+def _policy_inputs(shape, dev, old_log_probs, advantages, ref_log_probs, mask):
+    return (_same(old_log_probs, "old_log_probs", shape, dev, _F32_ONLY),
+            _same(advantages, "advantages", shape, dev, _F32_ONLY),
+            _opt_same(ref_log_probs, "ref_log_probs", shape, dev, _F32_ONLY),
+            _opt_same(mask, "mask", shape, dev, _WEIGHTS))
 
 
 def _k_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs=None, mask=None, clip_low=0.2, clip_high=0.2,
                    kl_coef=0.0, with_slopes=False):
     """-> loss, stats (mean KL, clipped share, 1 / sum of the weights), slopes or None"""
-    lp = _input(log_probs, "log_probs")
-    old, adv, ref, w = _policy_inputs(lp.shape, lp.device, old_log_probs, advantages, ref_log_probs, mask)
-    loss, stats = _f32((), lp.device), _f32(3, lp.device)
-    slopes = _f32(lp.shape, lp.device) if with_slopes else None
-    with _on_device(lp):
-        _check(_lib.b2_policy_loss(_stream(lp), _p(lp), _p(old), _p(adv), _opt(ref), _opt(w), _size(w), lp.numel(),
-                                   float(clip_low), float(clip_high), float(kl_coef), _p(loss), _p(stats),
-                                   _opt(slopes)))
+    lp = _log_probs(log_probs)
+    dev = lp.get_device()
+    old, adv, ref, w = _policy_inputs(lp.shape, dev, old_log_probs, advantages, ref_log_probs, mask)
+    loss, stats = lp.new_empty(()), lp.new_empty(3)
+    slopes = lp.new_empty(lp.shape) if with_slopes else None
+    _call(dev, _lib.b2_policy_loss, lp.data_ptr(), old.data_ptr(), adv.data_ptr(), _opt(ref), _opt(w), _size(w),
+          lp.numel(), float(clip_low), float(clip_high), float(kl_coef), loss.data_ptr(), stats.data_ptr(),
+          _opt(slopes))
     return loss, stats, slopes
 
 
 def _k_policy_loss_grad(grad_loss, stats, slopes):
-    gl = _scalar(grad_loss, "grad_loss", slopes.device)
-    out = torch.empty_like(slopes)
-    with _on_device(out):
-        _check(_lib.b2_policy_loss_grad(_stream(out), _p(gl), _p(stats), _p(slopes), out.numel(), _p(out)))
+    dev = slopes.get_device()
+    gl = _scalar(grad_loss, "grad_loss", dev)
+    out = slopes.new_empty(slopes.shape)
+    _call(dev, _lib.b2_policy_loss_grad, gl.data_ptr(), stats.data_ptr(), slopes.data_ptr(), out.numel(),
+          out.data_ptr())
     return out
 
 
@@ -815,14 +821,14 @@ def _k_policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log
                              clip_high=0.2, kl_coef=0.0, grad_loss=None):
     """-> loss, stats (mean KL, clipped share), grad_logits"""
     x, v = _logits(logits, "logits")
-    t = _ints(targets, "targets", x.shape[:-1], x.device)
-    old, adv, ref, w = _policy_inputs(t.shape, x.device, old_log_probs, advantages, ref_log_probs, mask)
-    gl = _scalar(grad_loss, "grad_loss", x.device)
-    loss, stats, grad = _f32((), x.device), _f32(2, x.device), _dense_like(x)
-    with _on_device(x):
-        _check(_lib.b2_policy_loss_with_grad(_stream(x), ctypes.byref(v), _p(t), t.element_size(), _p(old), _p(adv),
-                                             _opt(ref), _opt(w), _size(w), float(clip_low), float(clip_high),
-                                             float(kl_coef), _opt(gl), _p(loss), _p(stats), _p(grad)))
+    dev, lead = x.get_device(), x.shape[:-1]
+    t = _same(targets, "targets", lead, dev, _INTS)
+    old, adv, ref, w = _policy_inputs(lead, dev, old_log_probs, advantages, ref_log_probs, mask)
+    gl = _scalar(grad_loss, "grad_loss", dev)
+    loss, stats, grad = _f32(x, ()), _f32(x, 2), x.new_empty(x.shape)
+    _call(dev, _lib.b2_policy_loss_with_grad, ctypes.byref(v), t.data_ptr(), t.element_size(), old.data_ptr(),
+          adv.data_ptr(), _opt(ref), _opt(w), _size(w), float(clip_low), float(clip_high), float(kl_coef), _opt(gl),
+          loss.data_ptr(), stats.data_ptr(), grad.data_ptr())
     return loss, stats, grad
 
 
@@ -896,7 +902,18 @@ def _apply(op_type: str, kernel, inputs, attrs, nondiff=()):
 
 # The losses' gradients need more than an op's inputs and outputs (the rows'
 # softmax statistics, the slopes of sequences and tokens), so each is an
-# autograd node of its own instead of a registered gradient function.
+# autograd node of its own instead of a registered gradient function.  They are
+# differentiable once: a backward pass that is itself recorded (create_graph) gets
+# an error node, any other one goes straight to the kernel.
+
+def _once(backward):
+    recorded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return staticmethod(run)
+
 
 class _TokenLogProbsNode(torch.autograd.Function):
     @staticmethod
@@ -905,8 +922,7 @@ class _TokenLogProbsNode(torch.autograd.Function):
         ctx.save_for_backward(logits, targets, stats)
         return out
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         logits, targets, stats = ctx.saved_tensors
         return _k_token_log_probs_grad(grad, logits, targets, stats), None
@@ -920,8 +936,7 @@ class _DistillationNode(torch.autograd.Function):
         ctx.temperature = temperature
         return loss
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad):
         logits, ids, y, weights, stats = ctx.saved_tensors
         return _k_distillation_loss_grad(logits, ids, y, weights, ctx.temperature, stats, grad), None, None, None, None
@@ -937,8 +952,7 @@ class _PreferenceNode(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return loss, rewards
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad, _grad_rewards):
         if grad is None:
             return (None,) * 6
@@ -956,12 +970,12 @@ class _PolicyNode(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return loss, stats
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad, _grad_stats):
         if grad is None:
             return (None,) * 8
-        return (_k_policy_loss_grad(grad, *ctx.saved_tensors),) + (None,) * 7
+        stats, slopes = ctx.saved_tensors
+        return _k_policy_loss_grad(grad, stats, slopes), None, None, None, None, None, None, None
 
 
 def _differentiable(t) -> bool:
