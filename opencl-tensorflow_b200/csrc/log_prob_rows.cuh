@@ -440,12 +440,16 @@ __device__ __forceinline__ float class_q(const Teacher& t, int k, int top, int f
 
 // ------------------------------------------------------------ a row's end
 
-// log s to 3e-8: the exponent's part in 64 bits, where logf alone would round a
-// sum of ten to 5e-7.
+// log of a row's sum.  The exponent's part is added in 64 bits, where logf alone
+// would round a sum of ten to 5e-7.  ex2.approx gives 5.0e-8 too little on average
+// (measured on 2^20 arguments in each of [-1, 0], [-4, -2], [-24, -12]) for all but
+// the largest value's 2^0, which over the tokens of a sequence would add up;
+// the mean is put back.
 __device__ __forceinline__ double log_of(float s) {
-  const int e = (__float_as_int(s) >> 23) - 127;  // s is 0, inf, NaN or at least 2^-126 here
-  if (e < -126 || e > 127) return (double)logf(s);
-  return fma((double)e, M_LN2, (double)logf(__int_as_float(__float_as_int(s) - (e << 23))));
+  const int e = (__float_as_int(s) >> 23) - 127;
+  if (!(s >= 1.0f && e <= 127)) return (double)logf(s);  // NaN, inf, a row without a value
+  return fma((double)e, M_LN2, (double)logf(__int_as_float(__float_as_int(s) - (e << 23)))) +
+         (double)(5.0e-8f * (1.0f - __frcp_rn(s)));
 }
 
 __device__ __forceinline__ float log_prob(float x, const Stat& st) { return (float)((double)(x - st.m) - log_of(st.s)); }
@@ -661,18 +665,18 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps == 8 ? 5 : 3) long_ke
 // -------------------------------------------------------------- whole rows
 
 // Many rows: each group of kGroup threads has whole rows, one after the other.
-// kA: pass 1 (statistics and loss), kB: pass 2 (the gradient).  With both, pass 2
-// of a row and pass 1 of the group's next row run vector by vector in turn:
-// reads and writes reach HBM evenly mixed, where CTAs that began together would
-// all read and then all write (a write alone gets 3.8 TB/s, mixed with as
-// many reads 6.5 together), and the next row's loads hide the first one's end.
+// kA: pass 1 (statistics and loss), kB: pass 2 (the gradient).  What a row's end
+// needs of memory is loaded while the row before it is worked on.  Short rows
+// are bound by the instructions of a row's end (some 300 a warp), so as few
+// threads as keep the SMs full share one: with 8 lanes a row instead of 32 the
+// forward of 131072 x 2000 bf16 takes 106 us instead of 151 (floor 80).
 template <int kGroup>
 constexpr int cta_threads() {
   return kGroup <= 32 ? 256 : kGroup;
 }
 template <bool kA, bool kB>
 constexpr int resident_threads() {
-  return kA && kB ? 1024 : 1536;  // on an SM: 64 or 42 registers each
+  return kB ? 1024 : 1536;  // on an SM: more writing streams are slower (65536 x 4000 bf16: 182 us, 1536 threads 227)
 }
 
 template <class T, int kMode, int kGroup, bool kA, bool kB>
@@ -859,6 +863,10 @@ int launch_rows_as(cudaStream_t s, RowArgs a, const DeviceInfo* d, const char* w
     while (a.filter_words < 128 && a.filter_words * 4 < a.top) a.filter_words *= 2;
     a.teacher_bytes = (int)ceil_div(4 * (2 * a.filter_words + 3 * a.top), 16) * 16;
   }
+  const bool fill8 = a.rows * 8 >= sms * resident, fill32 = a.rows * 32 >= sms * resident;
+  // Forward alone: lanes of a warp keep up to rows of 16384 values, when there are twice as many as run at once.
+  if (!kB && a.classes > 4096 && a.classes <= 16384 && a.rows * 32 >= 2 * sms * resident && a.teacher_bytes <= 4096)
+    return launch_groups<T, kMode, 32, kA, kB>(s, a, resident / 256, d, what);
   if (a.classes >= kLongRow / (int64_t)sizeof(T) || (a.rows <= 2 * sms && a.classes >= 4096)) {
     // A cluster for a row whose slice L2 would not keep, and, for few rows, while
     // there are fewer CTAs than SMs and a slice keeps 2048 values.
@@ -875,10 +883,9 @@ int launch_rows_as(cudaStream_t s, RowArgs a, const DeviceInfo* d, const char* w
       return launch_long<T, kMode, kStep, 8>(s, a, ctas, what);
     }
   }
-  // As few threads a row as keep the SMs full, so that each has many values
-  // for its share of the row's end.
-  const bool fill8 = a.rows * 8 >= sms * resident, fill32 = a.rows * 32 >= sms * resident;
-  if (a.classes <= 1024 && fill8 && a.teacher_bytes <= 512)
+  // As few threads a row as keep the SMs full; where each writes, 8 lanes' 128
+  // bytes a row are too small a piece of longer rows.
+  if (a.classes <= (!kB ? 4096 : kA ? 2048 : 1024) && fill8 && a.teacher_bytes <= 512)
     return launch_groups<T, kMode, 8, kA, kB>(s, a, resident / 256, d, what);
   if ((a.classes <= 1024 || (fill32 && a.classes <= 8192)) && a.teacher_bytes <= 4096)
     return launch_groups<T, kMode, 32, kA, kB>(s, a, resident / 256, d, what);
