@@ -421,10 +421,11 @@ int b2_token_log_probs_grad(b2_stream_t stream, const b2_logits_t* logits,
                             void* grad_logits);
 
 /* Distillation from a teacher's `top` (1 to 1024) entries per row: classes
- * teacher_ids [rows, top] and their logits teacher_logits [rows, top].  With
- * q[r] the softmax of the row's teacher logits / temperature over the entries
- * whose class is not ignored and whose logit is not -inf, and P[r] the softmax
- * of the row's scores / temperature over all classes:
+ * teacher_ids [rows, top] and their logits teacher_logits [rows, top], at a
+ * temperature in [1e-30, 1e30].  With q[r] the softmax of the row's teacher
+ * logits / temperature over the entries whose class is not ignored and whose
+ * logit is not -inf, and P[r] the softmax of the row's scores / temperature over
+ * all classes:
  *   l[r] = temperature^2 * sum_k q[r,k] (log q[r,k] - log P[r, id[r,k]])
  *   *loss = sum_r w[r] l[r] / sum_r w[r]           (0 when the weights sum to 0)
  * A class may be repeated in a row; l[r] = 0 for a row without entries.

@@ -206,7 +206,8 @@ __global__ void __launch_bounds__(kTokenThreads)
     }
     const int64_t seq = lo - 1;
     const float w = weight_at(A.mask, A.mask_bytes, n);
-    grad[n] = seq >= 0 && seq < 2 * A.pairs && w != 0.0f ? gl * slopes[seq] * w : 0.0f;
+    const bool inside = seq >= 0 && seq < 2 * A.pairs && w != 0.0f;
+    grad[n] = inside ? gl * slopes[seq] * w : 0.0f;
   }
 }
 
@@ -401,7 +402,7 @@ static int distill_args(const b2_logits_t* logits, const void* teacher_ids, int 
              (long long)top);
   B2_REQUIRE(teacher_dtype == B2_FLOAT32 || teacher_dtype == B2_FLOAT16 || teacher_dtype == B2_BFLOAT16,
              "%s: teacher_logits must be float32, float16 or bfloat16", what);
-  B2_REQUIRE(temperature > 0.0 && std::isfinite(temperature), "%s: temperature must be positive and finite", what);
+  B2_REQUIRE(temperature >= 1e-30 && temperature <= 1e30, "%s: temperature must be in [1e-30, 1e30]", what);
   B2_REQUIRE(teacher_ids != nullptr && teacher_logits != nullptr, "%s: null pointer", what);
   a->ids = teacher_ids;
   a->ids_bytes = id_bytes;

@@ -218,8 +218,21 @@ __device__ __forceinline__ void add_edges(Stat& st, const T* __restrict__ row, c
   if (sp.tail + g < n) add_value(st, Pack<T>::one(row[sp.tail + g]), c);
 }
 
+// A vector of scores.  kAgain: it is read again, so it may stay in L1 (without
+// that pass 2 of 4096 x 128000 bf16 takes 100 us more); else it passes L1 by (the
+// forward of that then takes 162 us instead of 166).
+template <bool kAgain>
+__device__ __forceinline__ uint4 load_vector(const uint4* p) {
+  if (kAgain) return __ldg(p);
+  uint4 u;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+               : "l"(p));
+  return u;
+}
+
 // The vectors of a slice that thread g of kGroup adds up.
-template <class T, int kGroup>
+template <class T, int kGroup, bool kAgain>
 __device__ __forceinline__ Stat vectors_part(const T* __restrict__ row, const Span& sp, int g, float c) {
   Stat st{-INFINITY, 0.0f};
   const uint4* __restrict__ v = reinterpret_cast<const uint4*>(row + sp.head);
@@ -227,23 +240,23 @@ __device__ __forceinline__ Stat vectors_part(const T* __restrict__ row, const Sp
   for (; i + (kBatch - 1) * kGroup < sp.nvec; i += kBatch * kGroup) {
     uint4 u[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) u[k] = __ldg(v + i + k * kGroup);
+    for (int k = 0; k < kBatch; ++k) u[k] = load_vector<kAgain>(v + i + k * kGroup);
     add_vectors<T, kBatch>(st, u, c);
   }
   if (i < sp.nvec) {  // what is left, together
     uint4 u[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) u[k] = i + k * kGroup < sp.nvec ? __ldg(v + i + k * kGroup) : empty_vector<T>();
+    for (int k = 0; k < kBatch; ++k) u[k] = i + k * kGroup < sp.nvec ? load_vector<kAgain>(v + i + k * kGroup) : empty_vector<T>();
     add_vectors<T, kBatch>(st, u, c);
   }
   return st;
 }
 
 // The part of a slice that thread g of kGroup adds up.
-template <class T, int kGroup>
+template <class T, int kGroup, bool kAgain>
 __device__ __forceinline__ Stat slice_part(const T* __restrict__ row, int n, int g, float c) {
   const Span sp = span_of(row, n);
-  Stat st = vectors_part<T, kGroup>(row, sp, g, c);
+  Stat st = vectors_part<T, kGroup, kAgain>(row, sp, g, c);
   add_edges(st, row, sp, n, g, c);
   return st;
 }
@@ -452,7 +465,9 @@ __device__ __forceinline__ double log_of(float s) {
          (double)(5.0e-8f * (1.0f - __frcp_rn(s)));
 }
 
-__device__ __forceinline__ float log_prob(float x, const Stat& st) { return (float)((double)(x - st.m) - log_of(st.s)); }
+__device__ __forceinline__ float log_prob(float x, const Stat& st) {
+  return (float)((double)x - (double)st.m - log_of(st.s));
+}
 
 // The lanes' sum over the row's teacher of q (log q - log P), times the weight and T^2.
 template <int kLanes>
@@ -464,8 +479,8 @@ __device__ __forceinline__ double distill_row(const RowArgs& A, int64_t r, int l
     const float q = t.q[k];
     if (t.ids[k] < 0 || q == 0.0f) continue;
     const float y = teacher_at(A.teacher, A.teacher_dtype, r * A.top + k);
-    const double log_q = (double)(y - ymax) * inv_t - (double)log_sum_q;
-    sum += (double)q * (log_q - ((double)(t.x[k] - st.m) * inv_t - log_s));
+    const double log_q = ((double)y - (double)ymax) * inv_t - (double)log_sum_q;
+    sum += (double)q * (log_q - (((double)t.x[k] - (double)st.m) * inv_t - log_s));
   }
   return (double)w * lanes_sum<kLanes>(sum) * ((double)A.temperature * (double)A.temperature);
 }
@@ -538,13 +553,14 @@ __device__ __forceinline__ float unit_share(const RowArgs& A) {
 // write.  What costs is the time between the passes, which other CTAs of the SM
 // have to fill, and the rows that are between their passes: they have to stay in
 // L2 beside the writes.  Measured at 4096 x 128000 bf16 (floors 160 and 320 us):
-//   forward, 8 warps x 5 CTAs an SM: 166 us;  12 x 3: 173;  16 x 2: 186.
+//   forward, 8 warps x 5 CTAs an SM: 162 us;  8 x 6: 178;  12 x 3: 173;  16 x 2: 186.
 //   gradient alone, 12 x 3: 331 us;  8 x 5: 338;  16 x 2: 329.
-//   both, slices of 140 KB, 16 x 3: 396 us;  12 x 3: 411;  8 x 5: 453; whole rows
-//   of 256 KB, 16 x 3: 450.  Rows of 64 KB (8192 x 32000) 8 x 5: 202;  16 x 3: 213.
-// Slower were: slices held in shared memory between the passes (456), persistent
-// CTAs (444), pass 1 of the next row beside pass 2 of this one from a ring of
-// bulk copies (408 to 500), and both passes as tasks of other CTAs (568).
+//   both, slices of 140 KB, 16 x 3: 390 us;  12 x 3: 411;  8 x 5: 453; whole rows
+//   of 256 KB, 16 x 3: 443.  Rows of 64 KB (8192 x 32000) 8 x 6: 198;  16 x 3: 213;
+//   of 32 KB (16384 x 16000) 8 x 6: 196;  8 x 5: 226;  16 x 3: 264.
+// Slower at 4096 x 128000 were: slices held in shared memory between the passes
+// (456), persistent CTAs (444), pass 1 of the next row beside pass 2 of this one
+// from a ring of bulk copies (408 to 500), both passes as tasks of other CTAs (568).
 enum Pass {
   kForward,   // pass 1: statistics and loss
   kBackward,  // pass 2 with statistics from an earlier call
@@ -552,7 +568,7 @@ enum Pass {
 };
 
 template <class T, int kMode, int kPass, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps + 32, kWarps == 8 ? 5 : 3) long_kernel(const __grid_constant__ RowArgs A) {
+__global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kStep ? 6 : 5) long_kernel(const __grid_constant__ RowArgs A) {
   constexpr bool kStats = kPass != kBackward, kGrad = kPass != kForward;
   constexpr int kThreads = 32 * kWarps;
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -564,7 +580,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps == 8 ? 5 : 3) long_ke
   const bool helper = warp == kWarps;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t r = (int64_t)blockIdx.x / ranks;
+  const int64_t r = blockIdx.x / (unsigned)ranks;
   const T* row = row_at<T>(A, r);
   const int begin = min(A.classes, rank * A.slice), n = min(A.classes - begin, A.slice);
   const T* mine = row + begin;
@@ -604,7 +620,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps == 8 ? 5 : 3) long_ke
       share = w * unit_share(A);
     }
   } else if (kStats) {
-    st = slice_part<T, kThreads>(mine, n, g, A.c);
+    st = slice_part<T, kThreads, kGrad>(mine, n, g, A.c);
     st = lanes_merge<32>(st, A.c);
     if (lane == 0) part[warp] = st;
   }
@@ -742,7 +758,7 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kA, kB
   int buf = 0;
   Ahead now = look(r), next = look(r + step);
   Begun row = begin(r, now, 0);
-  if (kA && now.counts) row.st = slice_part<T, kGroup>(row_at<T>(A, r), n, g, A.c);
+  if (kA && now.counts) row.st = slice_part<T, kGroup, kB>(row_at<T>(A, r), n, g, A.c);
   if (kA) {
     row.st = lanes_merge<kLanes>(row.st, A.c);
     if (kCta && lane == 0) part[0][threadIdx.x >> 5] = row.st;
@@ -793,9 +809,9 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kA, kB
       T* out = static_cast<T*>(A.grad) + r * n;
       if (!writes) zero_slice<T, kGroup>(out, n, g);
       if (writes) write_slice<T, kGroup>(x, out, n, g, row.st.m, A.c, factor * inv_s);
-      if (kA && next.counts) begun.st = slice_part<T, kGroup>(row_at<T>(A, rn), n, g, A.c);
+      if (kA && next.counts) begun.st = slice_part<T, kGroup, kB>(row_at<T>(A, rn), n, g, A.c);
     } else if (next.counts) {
-      begun.st = slice_part<T, kGroup>(row_at<T>(A, rn), n, g, A.c);
+      begun.st = slice_part<T, kGroup, kB>(row_at<T>(A, rn), n, g, A.c);
     }
     if (kA) {
       begun.st = lanes_merge<kLanes>(begun.st, A.c);

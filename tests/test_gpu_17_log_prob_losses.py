@@ -518,6 +518,75 @@ def test_policy_loss_with_grad(otf, rows, classes, dtype):
     close(got[3], d, 2 * (tol + moved), "gradient by parts")
 
 
+# --------------------------------------------------- every way a row is shared
+
+# 8 lanes a row, a warp, a CTA, a cluster; forward alone, gradient alone, both in one call; rows that start on a 16-byte
+# border and rows that do not
+MANY = [(30011, 37, "f32"), (30000, 64, "bf16"), (29000, 1500, "bf16"), (29000, 3001, "f16"), (15000, 5003, "bf16"),
+        (15000, 9001, "f16"), (1200, 2100, "f32"), (700, 16000, "bf16"), (400, 30001, "f16"), (160, 60000, "bf16"),
+        (151, 131075, "f32"), (9, 400000, "bf16"), (1, 700001, "f32")]
+
+
+@pytest.mark.parametrize("rows,classes,dtype", MANY)
+def test_many_rows(otf, rows, classes, dtype):
+    x, t = scores(rows, classes, dtype, rows)
+    t[::5] = -100
+    g = torch.randn(rows, device="cuda")
+    ids, y = teacher(x, min(9, classes), 3)
+    w = torch.rand(rows, device="cuda") + 0.5
+    if rows > 1:
+        w[rows // 2] = 0.0
+        x[rows // 2] = math.nan
+        t[rows // 2] = -1
+    leaf = x.clone().requires_grad_()
+    lp = otf.losses.token_log_probs(leaf, t)
+    lp_grad, = torch.autograd.grad(lp, leaf, g)
+    scale = torch.tensor(float(rows), device="cuda")
+    loss, grad = otf.losses.distillation_loss_with_grad(x, ids, y, weights=w, temperature=1.5, grad_loss=scale)
+    two = otf.losses.distillation_loss(leaf, ids, y, weights=w, temperature=1.5)
+    two_grad, = torch.autograd.grad(two, leaf, scale)
+    adv = torch.randn(rows, device="cuda")
+    old = lp.detach() + 0.1 * torch.randn(rows, device="cuda")
+    pol = otf.losses.policy_loss_with_grad(x, t, old, adv, mask=w, grad_loss=scale)
+    pol_grad, = torch.autograd.grad(otf.losses.policy_loss(otf.losses.token_log_probs(leaf, t), old, adv, mask=w)[0], leaf,
+                                    scale)
+    total, loss_sum, loss_off = float(w.double().sum()), 0.0, 0.0
+    step = max(1, (1 << 25) // classes)
+    for a in range(0, rows, step):
+        r = slice(a, min(rows, a + step))
+        want, valid = ref_log_probs(x[r], t[r])
+        want = want.masked_fill(~valid, 0.0)
+        _, rel_s, _ = parts(x[r].nan_to_num() if rows > 1 else x[r])
+        close(lp.detach()[r], want, rel_s[:, 0] + 2 * U * want.abs() + U, "log-probabilities")
+        want, tol = ref_log_probs_grad(x[r].nan_to_num(nan=0.0, neginf=-math.inf), t[r], g[r], x.dtype)
+        close(lp_grad[r], want, tol, "their gradient")
+        part = float(w[r].double().sum())
+        if part == 0.0:
+            assert not grad[r].any()
+            continue
+        l, d, l_off, tol = ref_distill(x[r].nan_to_num(nan=0.0, neginf=-math.inf), ids[r], y[r], w[r], 1.5, rows * part / total)
+        loss_sum += float(l) * part / total
+        loss_off += float(l_off) * part / total
+        close(grad[r], d, tol, "gradient in one call")
+        close(two_grad[r], d, tol, "gradient")
+        # both forms of the policy loss are within their tolerance of the same value: the log-probability's error
+        # times how fast the slope moves with it, and the gradient's own
+        p = parts(x[r].nan_to_num(nan=0.0, neginf=-math.inf))[2]
+        near = (w[r, None] * adv[r, None].abs() * 2 * rows / total).double()
+        close(pol[3][r], pol_grad[r], 2 * near * (p + 8 * rel_s + 20 * U) + 2 * torch.finfo(x.dtype).eps * pol_grad[r].double().abs()
+              + 2 * TINY[x.dtype], "policy gradient")
+    for got in (loss, two.detach()):
+        assert abs(float(got) - loss_sum) <= loss_off + 2 * U * abs(loss_sum)
+
+
+def test_no_token_counts(otf):
+    x, t = scores(40, 300, "f32", 1)
+    none = torch.zeros(40, dtype=torch.bool, device="cuda")
+    lp = torch.zeros(40, device="cuda")
+    got = otf.losses.policy_loss_with_grad(x, t, lp, lp + 1, ref_log_probs=lp, mask=none, kl_coef=1.0)
+    assert all(not o.any() for o in got)
+
+
 # ---------------------------------------------------------------- together
 
 def test_gradients_against_differences(otf):
