@@ -732,11 +732,11 @@ def _k_distillation_loss(logits, teacher_ids, teacher_logits, weights=None, temp
     ids, y, w = _teacher(x, dev, lead, teacher_ids, teacher_logits, weights)
     gl = _scalar(grad_loss, "grad_loss", dev)
     loss = _f32(x, ())
-    stats = _f32(x, 4 * (v.outer * v.inner) + 2) if with_stats else None
+    stats = _f32(x, 4 * (v.outer * v.inner) + 2)  # the call's workspace, too
     grad = x.new_empty(x.shape) if with_grad else None
     _call(dev, _lib.b2_distillation_loss, ctypes.byref(v), ids.data_ptr(), ids.element_size(), y.data_ptr(),
-          _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w), float(temperature), loss.data_ptr(), _opt(stats),
-          _opt(gl), _opt(grad))
+          _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w), float(temperature), loss.data_ptr(),
+          stats.data_ptr(), _opt(gl), _opt(grad))
     return (loss, stats) if with_stats else (loss, grad) if with_grad else loss
 
 

@@ -1,5 +1,5 @@
-"""One training step of a model built from this package: forward, MSE loss,
-backward through the registered gradients, data-parallel gradient averaging,
+"""One training step of a model built from this package: forward, loss (MSE, or
+any of ``losses``), backward through the registered gradients, data-parallel gradient averaging,
 Adam -- what ``model.compile(Adam(1e-3), "mse"); model.fit(...)`` runs per
 batch in the reference (README.md:188-196).  Loss and optimizer are this
 package's device kernels with Keras's formulas (``step_ops.opencl_mse_loss``,
@@ -277,8 +277,26 @@ class GradientAverager:
             off += n
 
 
+def _buffers_like(y):
+    """Static input buffers for targets that are a tensor or a tuple of tensors."""
+    return tuple(torch.empty_like(t) for t in y) if isinstance(y, tuple) else torch.empty_like(y)
+
+
+def _copy_into(buffers, y, non_blocking: bool = False) -> None:
+    pairs = zip(buffers, y) if isinstance(buffers, tuple) else ((buffers, y),)
+    for b, t in pairs:
+        if t.data_ptr() != b.data_ptr():
+            b.copy_(t, non_blocking=non_blocking)
+
+
 class TrainStep:
-    """fwd + MSE + bwd + gradient averaging + Adam for ``model`` on (x, y).
+    """fwd + loss + bwd + gradient averaging + Adam for ``model`` on (x, y).
+
+    ``loss(output, y)``: the mean squared error by default; any function of the
+    model's output and the targets that returns a device scalar, or a tuple
+    that begins with one, made of differentiable ops that a CUDA graph can
+    hold (the ones of ``losses``, for instance).  ``y`` is what it needs: a tensor
+    or a tuple of tensors, e.g. a teacher's (classes, logits).
 
     ``reserved_sms``: with more than one rank, SMs kept free of the library's
     persistent tensor-core kernels so that NCCL's all-reduce kernels (and the
@@ -288,8 +306,9 @@ class TrainStep:
     are about ``B2_BUCKET_BYTES`` (default 4 MiB) each."""
 
     def __init__(self, model: torch.nn.Module, lr: float = 1e-3, graphed: bool = True, warmup: int = 3,
-                 group=None, reserved_sms: int | None = None):
+                 group=None, reserved_sms: int | None = None, loss=None):
         self.model = model
+        self.loss = mse if loss is None else loss
         self.params = [p for p in model.parameters() if p.requires_grad]
         dev = self.params[0].device
         bucket = int(os.environ.get("B2_BUCKET_BYTES", str(4 << 20)))
@@ -334,7 +353,9 @@ class TrainStep:
 
     def _eager(self, x, y):
         self.zero_grad()
-        loss = mse(self.model(x, training=True), y)
+        loss = self.loss(self.model(x, training=True), y)
+        if isinstance(loss, tuple):
+            loss = loss[0]
         self.avg.begin()
         loss.backward()
         if len(self.opts) == 2:
@@ -352,9 +373,9 @@ class TrainStep:
 
     def _capture(self, x, y):
         self.static_x = torch.empty_like(x)
-        self.static_y = torch.empty_like(y)
+        self.static_y = _buffers_like(y)
         self.static_x.copy_(x)
-        self.static_y.copy_(y)
+        _copy_into(self.static_y, y)
         side = torch.cuda.Stream(device=x.device)
         side.wait_stream(torch.cuda.current_stream(x.device))
         with torch.cuda.stream(side):
@@ -375,8 +396,7 @@ class TrainStep:
         else:
             if x.data_ptr() != self.static_x.data_ptr():
                 self.static_x.copy_(x, non_blocking=True)
-            if y.data_ptr() != self.static_y.data_ptr():
-                self.static_y.copy_(y, non_blocking=True)
+            _copy_into(self.static_y, y, non_blocking=True)
         self.graph.replay()
         return self.static_loss
 
@@ -392,9 +412,9 @@ class TrainStep:
             return self.static_x, self.static_y
         if self.graph1 is None:
             self.static_x1 = torch.empty_like(self.static_x)
-            self.static_y1 = torch.empty_like(self.static_y)
+            self.static_y1 = _buffers_like(self.static_y)
             self.static_x1.copy_(self.static_x)
-            self.static_y1.copy_(self.static_y)
+            _copy_into(self.static_y1, self.static_y)
             torch.cuda.current_stream(self.static_x.device).synchronize()
             self.graph1 = torch.cuda.CUDAGraph()
             self.zero_grad()

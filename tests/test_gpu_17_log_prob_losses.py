@@ -726,3 +726,69 @@ def test_dense_head_distilled(otf):
     assert abs(float(loss) - float(ref)) <= 1e-5 * abs(float(ref))
     for got, want in ((w.grad, w64.grad), (b.grad, b64.grad)):
         assert float((got - want).norm() / want.norm()) <= 2e-5
+
+
+class _Classifier(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        from opencl_tf.layers import OpenCLDense
+        self.hidden, self.out = OpenCLDense(48), OpenCLDense(1021)
+        self.hidden.build((1, 30))
+        self.out.build((1, 48))
+
+    def forward(self, x, training=None):
+        return self.out(self.hidden.forward_relu(x))
+
+
+@pytest.mark.parametrize("kind", ["distillation", "likelihood"])
+def test_train_step_with_a_loss(otf, kind):
+    """TrainStep on one of the losses: captured in a graph it does what it does eagerly, bit for bit, over steps with
+    new inputs; and the first step's gradients are the definition's."""
+    from opencl_tf.train import TrainStep
+
+    def batch(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x = torch.randn(64, 30, generator=g, device="cuda")
+        if kind == "likelihood":
+            return x, torch.randint(0, 1021, (64,), generator=g, device="cuda")
+        top = torch.randn(64, 1021, generator=g, device="cuda").topk(8, 1)
+        return x, (top.indices, top.values)
+
+    def loss(output, y):
+        if kind == "likelihood":
+            return -otf.losses.token_log_probs(output, y).mean()
+        return otf.losses.distillation_loss(output, *y, temperature=2.0)
+
+    def run(graphed):
+        torch.manual_seed(3)
+        model = _Classifier().cuda()
+        first = [p.detach().clone() for p in model.parameters()]
+        step = TrainStep(model, graphed=graphed, warmup=1, loss=loss)
+        if graphed:  # the capture's warm-up takes steps of its own: back to the start
+            step(*batch(0))
+            with torch.no_grad():
+                for p, f in zip(model.parameters(), first):
+                    p.copy_(f)
+                for o in step.opts:
+                    o.iterations.zero_()
+                    for slot in (*o.m, *o.v):
+                        slot.zero_()
+        losses = [step(*batch(s)).clone() for s in (1, 2, 3)]
+        return losses, [p.detach().clone() for p in model.parameters()]
+
+    a, b = run(True), run(False)
+    for x, y in zip((*a[0], *a[1]), (*b[0], *b[1])):
+        assert torch.equal(x, y)
+    torch.manual_seed(3)
+    model = _Classifier().cuda()
+    x, y = batch(1)
+    loss(model(x), y).backward()
+    params = [p.detach().double().requires_grad_() for p in model.parameters()]
+    h = torch.relu(x.double() @ params[0] + params[1]) @ params[2] + params[3]
+    if kind == "likelihood":
+        ref = -torch.log_softmax(h, 1).gather(1, y[:, None]).mean()
+    else:
+        ref = ref_distill(h, *y, None, 2.0)[0]
+    for got, want in zip(model.parameters(), torch.autograd.grad(ref, params)):
+        # the products' fp32 tolerance, 5e-6 of the largest value each way
+        assert float((got.grad - want).norm() / want.norm()) <= 2e-5
