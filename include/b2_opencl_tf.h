@@ -384,8 +384,8 @@ int b2_adam_update(b2_stream_t stream, int num_tensors, float* const* params,
  * scores over many classes is trained on chosen classes, on another network's
  * top answers, on pairs of answers or on rewards.
  *
- * Scores ("logits") are float32, float16 or bfloat16 rows of `classes`
- * adjacent values; row (i, j), i < outer, j < inner, starts at element
+ * Scores ("logits") are float32, float16 or bfloat16 rows of `classes` (1 to
+ * 2^30) adjacent values; row (i, j), i < outer, j < inner, starts at element
  * i * outer_stride + j * inner_stride of `data` (so the rows of a larger
  * tensor, e.g. every position but the last of a batch of sequences, need no
  * copy).  Rows are numbered i * inner + j; gradients of scores are dense

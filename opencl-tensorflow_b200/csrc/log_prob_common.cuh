@@ -29,7 +29,8 @@ struct RowArgs {
   int filter_words;   // of each of a teacher's two bit filters, a power of two
   int teacher_bytes;  // shared memory of a row's teacher
   float c;  // log2(e) / temperature
-  float temperature, inv_t;
+  float temperature;
+  double inv_t;
   float2* stats;   // [rows] (m, s): written by pass 1 unless null, read by pass 2 alone
   void* grad;      // [rows, classes] dense; null: no pass 2
   // the chosen classes

@@ -316,7 +316,7 @@ int row_args(const b2_logits_t* x, const char* what, RowArgs* a) {
   B2_REQUIRE(x->dtype == B2_FLOAT32 || x->dtype == B2_FLOAT16 || x->dtype == B2_BFLOAT16,
              "%s: logits must be float32, float16 or bfloat16", what);
   B2_REQUIRE(x->outer >= 0 && x->inner >= 0, "%s: negative number of rows", what);
-  B2_REQUIRE(x->classes >= 1 && x->classes < kMaxInt32, "%s: classes must be in [1, 2^31 - 2], got %lld", what,
+  B2_REQUIRE(x->classes >= 1 && x->classes <= (1 << 30), "%s: classes must be in [1, 2^30], got %lld", what,
              (long long)x->classes);
   B2_REQUIRE(x->inner == 0 || x->outer <= kMaxInt32 / x->inner, "%s: too many rows", what);
   B2_REQUIRE(x->outer * x->inner == 0 || x->data != nullptr, "%s: null logits", what);
@@ -327,7 +327,8 @@ int row_args(const b2_logits_t* x, const char* what, RowArgs* a) {
   a->outer_stride = x->outer_stride;
   a->inner_stride = x->inner_stride;
   a->classes = (int)x->classes;
-  a->temperature = a->inv_t = 1.0f;
+  a->temperature = 1.0f;
+  a->inv_t = 1.0;
   a->c = (float)M_LOG2E;
   return B2_OK;
 }
@@ -412,7 +413,7 @@ static int distill_args(const b2_logits_t* logits, const void* teacher_ids, int 
   a->weights = weights;
   a->weight_bytes = weight_bytes;
   a->temperature = (float)temperature;
-  a->inv_t = (float)(1.0 / temperature);
+  a->inv_t = 1.0 / temperature;
   a->c = (float)(M_LOG2E / temperature);
   return B2_OK;
 }

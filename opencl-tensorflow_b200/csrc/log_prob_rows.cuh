@@ -208,7 +208,9 @@ __device__ __forceinline__ Span span_of(const T* p, int n) {
 // A vector of -inf.
 template <class T>
 __device__ __forceinline__ uint4 empty_vector() {
-  const uint32_t w = std::is_same<T, float>::value ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  const uint32_t w = std::is_same<T, float>::value    ? 0xff800000u
+                     : std::is_same<T, __half>::value ? 0xfc00fc00u
+                                                      : 0xff80ff80u;
   return make_uint4(w, w, w, w);
 }
 
@@ -246,7 +248,8 @@ __device__ __forceinline__ Stat vectors_part(const T* __restrict__ row, const Sp
   if (i < sp.nvec) {  // what is left, together
     uint4 u[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) u[k] = i + k * kGroup < sp.nvec ? load_vector<kAgain>(v + i + k * kGroup) : empty_vector<T>();
+    for (int k = 0; k < kBatch; ++k)
+      u[k] = i + k * kGroup < sp.nvec ? load_vector<kAgain>(v + i + k * kGroup) : empty_vector<T>();
     add_vectors<T, kBatch>(st, u, c);
   }
   return st;
@@ -399,10 +402,10 @@ __device__ __forceinline__ int filter_word(int id, int filter_words) { return (i
 // A row's lanes lay out its teacher: softmax over the entries whose class
 // lies in the row and whose logit is not -inf.  Returns false when there is none.
 template <class T, int kLanes>
-__device__ __forceinline__ bool load_teacher(const RowArgs& A, int64_t r, const T* row, int lane, const Teacher& t, float* ymax,
-                             float* log_sum) {
+__device__ __forceinline__ bool load_teacher(const RowArgs& A, int64_t r, const T* row, int lane, const Teacher& t,
+                                             float* ymax, float* sum_q) {
   const int64_t base = r * A.top;
-  const float inv_t = A.inv_t;
+  const float inv_t = (float)A.inv_t;
   for (int i = lane; i < A.filter_words; i += kLanes) t.seen[i] = t.again[i] = 0u;
   float mx = -INFINITY;
   bool nan = false;
@@ -437,7 +440,7 @@ __device__ __forceinline__ bool load_teacher(const RowArgs& A, int64_t r, const 
   for (int k = lane; k < A.top; k += kLanes) t.q[k] = t.q[k] / sum;
   __syncwarp(lanes_mask<kLanes>());
   *ymax = mx;
-  *log_sum = logf(sum);
+  *sum_q = sum;
   return true;
 }
 
@@ -453,33 +456,36 @@ __device__ __forceinline__ float class_q(const Teacher& t, int k, int top, int f
 
 // ------------------------------------------------------------ a row's end
 
-// log of a row's sum.  The exponent's part is added in 64 bits, where logf alone
-// would round a sum of ten to 5e-7.  ex2.approx gives 5.0e-8 too little on average
-// (measured on 2^20 arguments in each of [-1, 0], [-4, -2], [-24, -12]) for all but
-// the largest value's 2^0, which over the tokens of a sequence would add up;
-// the mean is put back.
+// log s of a sum of at least 1 that logf would round to 5e-7 (of ten): the exponent's part is added in 64 bits.
 __device__ __forceinline__ double log_of(float s) {
   const int e = (__float_as_int(s) >> 23) - 127;
   if (!(s >= 1.0f && e <= 127)) return (double)logf(s);  // NaN, inf, a row without a value
-  return fma((double)e, M_LN2, (double)logf(__int_as_float(__float_as_int(s) - (e << 23)))) +
-         (double)(5.0e-8f * (1.0f - __frcp_rn(s)));
+  return fma((double)e, M_LN2, (double)logf(__int_as_float(__float_as_int(s) - (e << 23))));
+}
+
+// log of a row's sum.  ex2.approx gives 5.0e-8 too little on average (measured
+// on 2^20 arguments in each of [-1, 0], [-4, -2], [-24, -12]) for all but the
+// largest value's 2^0, which over the tokens of a sequence would add up; the
+// mean is put back.
+__device__ __forceinline__ double log_row(float s) {
+  return log_of(s) + (double)(5.0e-8f * (1.0f - __frcp_rn(s)));
 }
 
 __device__ __forceinline__ float log_prob(float x, const Stat& st) {
-  return (float)((double)x - (double)st.m - log_of(st.s));
+  return (float)((double)x - (double)st.m - log_row(st.s));
 }
 
 // The lanes' sum over the row's teacher of q (log q - log P), times the weight and T^2.
 template <int kLanes>
 __device__ __forceinline__ double distill_row(const RowArgs& A, int64_t r, int lane, const Teacher& t, const Stat& st,
-                                              float ymax, float log_sum_q, float w) {
-  const double inv_t = A.inv_t, log_s = log_of(st.s);
+                                              float ymax, float sum_q, float w) {
+  const double inv_t = A.inv_t, log_s = log_row(st.s), log_q_sum = log_of(sum_q);
   double sum = 0.0;
   for (int k = lane; k < A.top; k += kLanes) {
     const float q = t.q[k];
     if (t.ids[k] < 0 || q == 0.0f) continue;
     const float y = teacher_at(A.teacher, A.teacher_dtype, r * A.top + k);
-    const double log_q = ((double)y - (double)ymax) * inv_t - (double)log_sum_q;
+    const double log_q = ((double)y - (double)ymax) * inv_t - log_q_sum;
     sum += (double)q * (log_q - (((double)t.x[k] - (double)st.m) * inv_t - log_s));
   }
   return (double)w * lanes_sum<kLanes>(sum) * ((double)A.temperature * (double)A.temperature);
@@ -568,7 +574,8 @@ enum Pass {
 };
 
 template <class T, int kMode, int kPass, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kStep ? 6 : 5) long_kernel(const __grid_constant__ RowArgs A) {
+__global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kStep ? 6 : 5)
+    long_kernel(const __grid_constant__ RowArgs A) {
   constexpr bool kStats = kPass != kBackward, kGrad = kPass != kForward;
   constexpr int kThreads = 32 * kWarps;
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -602,12 +609,12 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kS
   // ---- pass 1; the helper meanwhile fetches what the row's end needs
   const Teacher teacher = kMode == kDistill ? teacher_in(dyn, A.top, A.filter_words) : Teacher{};
   Stat st{-INFINITY, 0.0f};
-  float x_target = 0.0f, ymax = 0.0f, log_sum_q = 0.0f, share = 0.0f;
+  float x_target = 0.0f, ymax = 0.0f, sum_q = 0.0f, share = 0.0f;
   PolicyToken token{};
   bool real = true;
   if (helper) {
     if (kMode == kDistill) {
-      real = load_teacher<T, 32>(A, r, row, lane, teacher, &ymax, &log_sum_q);
+      real = load_teacher<T, 32>(A, r, row, lane, teacher, &ymax, &sum_q);
       if (lane == 0) {
         if (kGrad) factor_s = A.temperature * w * unit_share(A);
         real_s = real;
@@ -654,7 +661,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kS
     if (A.stats != nullptr && lane == 0) A.stats[r] = make_float2(st.m, st.s);
     if (kMode == kLogProb && lane == 0) A.log_probs[r] = log_prob(x_target, st);
     if (kMode == kDistill) {
-      const double loss = real ? distill_row<32>(A, r, lane, teacher, st, ymax, log_sum_q, w) : 0.0;
+      const double loss = real ? distill_row<32>(A, r, lane, teacher, st, ymax, sum_q, w) : 0.0;
       if (lane == 0) A.row_out[r] = loss;
     }
   }
@@ -731,7 +738,7 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kA, kB
     return teacher_in(dyn + (2 * group + buf) * A.teacher_bytes, A.top, A.filter_words);
   };
   struct Begun {  // a row whose end is near
-    float x_target, ymax, log_sum_q;
+    float x_target, ymax, sum_q;
     bool real;
     Stat st;
   };
@@ -744,7 +751,7 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kA, kB
       if (leader && b.real) b.x_target = Pack<T>::one(row[h.target]);
     } else if (leader) {
       __syncwarp(lanes_mask<kLanes>());  // the row that had this buffer is done with it
-      b.real = load_teacher<T, kLanes>(A, i, row, lane, teacher_of(buf), &b.ymax, &b.log_sum_q);
+      b.real = load_teacher<T, kLanes>(A, i, row, lane, teacher_of(buf), &b.ymax, &b.sum_q);
       if (kCta && lane == 0) real_s[buf] = b.real;
     }
     if (!kA) {
@@ -777,13 +784,14 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kA, kB
       } else if (kMode == kDistill) {
         if (kA && leader) {
           const double loss =
-              row.real ? distill_row<kLanes>(A, r, lane, teacher_of(buf), row.st, row.ymax, row.log_sum_q, now.w) : 0.0;
+              row.real ? distill_row<kLanes>(A, r, lane, teacher_of(buf), row.st, row.ymax, row.sum_q, now.w) : 0.0;
           if (lane == 0) A.row_out[r] = loss;
         }
         if (kB) factor = A.temperature * now.w * unit;
       } else {
         if (g == 0) {
-          const PolicyTerm t = policy_term(row.real ? log_prob(row.x_target, row.st) : 0.0f, policy_token(A, r), A.clip);
+          const float lp = row.real ? log_prob(row.x_target, row.st) : 0.0f;
+          const PolicyTerm t = policy_term(lp, policy_token(A, r), A.clip);
           store_policy(A, r, t, now.w);
           factor = -now.w * unit * t.slope;
           if (kCta) factor_s[buf] = factor;

@@ -49,7 +49,7 @@ def refused(rc, *words):
 
 
 BAD_SCORES = [(dict(dtype=3), "bfloat16"), (dict(dtype=-1), "bfloat16"), (dict(classes=0), "classes"),
-              (dict(classes=2 ** 31 - 1), "classes"), (dict(inner=-1), "negative"), (dict(outer=-1), "negative"),
+              (dict(classes=2 ** 30 + 1), "classes"), (dict(inner=-1), "negative"), (dict(outer=-1), "negative"),
               (dict(outer=2 ** 20, inner=2 ** 20), "too many rows"), (dict(data=None), "null")]
 
 
@@ -85,7 +85,7 @@ def test_bad_arguments():
     refused(distill(w=P, w_bytes=2), "weights")
     for top in (0, -1, 1025):
         refused(distill(top=top), "[1, 1024]")
-    for t in (0.0, -1.0, float("inf"), float("nan")):
+    for t in (0.0, -1.0, 1e-31, 1e31, float("inf"), float("nan")):
         refused(distill(t=t), "temperature")
 
     def preference(off=P, off_bytes=8, pairs=2, beta=0.1, eps=0.0, n=5, lp=P, loss=P, w=None, w_bytes=0):

@@ -7,7 +7,7 @@ sequences, graph capture, streams.
 Tolerances.  u = 2^-24 is half a step of fp32.  A row's exponent (x - m) * c has
 relative error 3u (difference, product, the constant c), so 2^that is off by
 3u |x - m| / T; ex2 adds 4u (2 ulp).  s is a sum of positive terms: at most
-kGroup-independent ``chain`` additions follow one another, each u.  With
+``chain`` additions follow one another, each u.  With
 D = sum_j p_j |x_j - m| / T the relative error of s is <= u (3 D + 4 + chain),
 and that of p_j <= u (3 |x_j - m| / T + 8) more.  A stored value adds half a step of its type."""
 from __future__ import annotations
@@ -27,9 +27,10 @@ TINY = {torch.float64: 0.0, torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -2
 
 def chain(classes):
     """Additions that follow one another in a row's sum: a thread's values
-    (batches of 32, then the batches), the warp's 5 + the CTA's 5 + the cluster's 5 merges of
-    one addition and two products each."""
-    per_thread = min(classes, max(32, -(-classes // 256)))
+    (batches of at most 32, then the batches), the warp's 5 + the CTA's 5 + the
+    cluster's 5 merges of one addition and two products each.  A thread has an eighth of a row of up to
+    4096 values at most, a 32nd of one of up to 16384, a 256th of a longer one."""
+    per_thread = -(-classes // (8 if classes <= 4096 else 32 if classes <= 16384 else 256))
     return 32 + per_thread // 32 + 16 + 45
 
 
@@ -644,7 +645,8 @@ def test_preference_step_in_a_graph(otf):
         ids = t.clamp(min=0)[:, None].expand(-1, 3).contiguous()
         both, dx = otf.losses.distillation_loss_with_grad(x, ids, torch.ones(21, 3, device="cuda"), weights=t >= 0)
         pl = otf.losses.policy_loss(lp, ref, ref, ref, kl_coef=0.1)
-        return loss, c, r, both, dx, *torch.autograd.grad(loss + pl[0], leaf)
+        fused = otf.losses.policy_loss_with_grad(x, t, ref, ref, ref, mask=t >= 0, kl_coef=0.1)
+        return loss, c, r, both, dx, *fused, *torch.autograd.grad(loss + pl[0], leaf)
 
     eager = [[o.clone() for o in step(*inputs(s))] for s in (1, 2, 3)]
     side = torch.cuda.Stream()
