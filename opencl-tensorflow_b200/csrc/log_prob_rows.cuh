@@ -221,8 +221,8 @@ __device__ __forceinline__ void add_edges(Stat& st, const T* __restrict__ row, c
 }
 
 // A vector of scores.  kAgain: it is read again, so it may stay in L1 (without
-// that pass 2 of 4096 x 128000 bf16 takes 100 us more); else it passes L1 by (the
-// forward of that then takes 162 us instead of 166).
+// that, loss and gradient of 4096 x 128000 bf16 take 100 us more); else it passes
+// L1 by (the forward of 131072 x 2000 then takes 103 us instead of 109).
 template <bool kAgain>
 __device__ __forceinline__ uint4 load_vector(const uint4* p) {
   if (kAgain) return __ldg(p);
@@ -559,7 +559,7 @@ __device__ __forceinline__ float unit_share(const RowArgs& A) {
 // write.  What costs is the time between the passes, which other CTAs of the SM
 // have to fill, and the rows that are between their passes: they have to stay in
 // L2 beside the writes.  Measured at 4096 x 128000 bf16 (floors 160 and 320 us):
-//   forward, 8 warps x 5 CTAs an SM: 162 us;  8 x 6: 178;  12 x 3: 173;  16 x 2: 186.
+//   forward, 8 warps x 5 CTAs an SM: 167 us;  8 x 6: 178;  12 x 3: 173;  16 x 2: 186.
 //   gradient alone, 12 x 3: 331 us;  8 x 5: 338;  16 x 2: 329.
 //   both, slices of 140 KB, 16 x 3: 390 us;  12 x 3: 411;  8 x 5: 453; whole rows
 //   of 256 KB, 16 x 3: 443.  Rows of 64 KB (8192 x 32000) 8 x 6: 198;  16 x 3: 213;
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kS
   const bool helper = warp == kWarps;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t r = blockIdx.x / (unsigned)ranks;
+  const int64_t r = (int64_t)blockIdx.x / ranks;
   const T* row = row_at<T>(A, r);
   const int begin = min(A.classes, rank * A.slice), n = min(A.classes - begin, A.slice);
   const T* mine = row + begin;
@@ -692,7 +692,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kS
 // needs of memory is loaded while the row before it is worked on.  Short rows
 // are bound by the instructions of a row's end (some 300 a warp), so as few
 // threads as keep the SMs full share one: with 8 lanes a row instead of 32 the
-// forward of 131072 x 2000 bf16 takes 106 us instead of 151 (floor 80).
+// forward of 131072 x 2000 bf16 takes 103 us instead of 151 (floor 80).
 template <int kGroup>
 constexpr int cta_threads() {
   return kGroup <= 32 ? 256 : kGroup;
