@@ -19,7 +19,7 @@ struct PolicyToken {
 };
 struct PolicyClip {
   double low, high;  // the ratio's range
-  float kl_coef;
+  double kl_coef;
 };
 struct RowArgs {
   const void* x;
@@ -73,28 +73,33 @@ __device__ __forceinline__ float weight_at(const void* w, int bytes, int64_t i) 
 }
 
 struct PolicyTerm {
-  float value, slope, kl;
+  double value;
+  float slope, kl;
   bool cut;
 };
 
 // One token's term of the clipped policy loss and its slope in the token's
-// log-probability, in 32 bits.  Only a ratio within 1e-5 of a border, where its
-// rounding could put it on the other side, is looked at again in 64; and
-// exp(d) - d - 1 is its series for |d| <= 1, where the subtraction would cancel.
+// log-probability.  kWide: the ratio is taken in 64 bits; else in 32, and only one
+// within 1e-5 of a border, where its rounding could put it on the other side, is
+// looked at again in 64.  The value is put together in 64 bits: advantages of both
+// signs cancel in the mean, and a border or coefficient rounded to 32 bits would
+// move all cut tokens' terms the same way.  exp(d) - d - 1 is its series for
+// |d| <= 1, where the subtraction would cancel.
+template <bool kWide>
 __device__ __forceinline__ PolicyTerm policy_term(float lp, const PolicyToken& t, const PolicyClip& c) {
   PolicyTerm p;
-  const float low = (float)c.low, high = (float)c.high, adv = t.advantage;
-  const float ratio = expf(lp - t.old_lp);
-  bool above = ratio > high, below = ratio < low;
-  if (fabsf(ratio - high) <= 1e-5f * high || fabsf(ratio - low) <= 1e-5f) {
+  const float adv = t.advantage;
+  const double ratio = kWide ? exp((double)lp - (double)t.old_lp) : (double)expf(lp - t.old_lp);
+  bool above = ratio > c.high, below = ratio < c.low;
+  if (!kWide && (fabs(ratio - c.high) <= 1e-5 * c.high || fabs(ratio - c.low) <= 1e-5)) {
     const double exact = exp((double)lp - (double)t.old_lp);
     above = exact > c.high;
     below = exact < c.low;
   }
   p.cut = (adv > 0.0f && above) || (adv < 0.0f && below);
   // Where it is not cut, the unclipped term is the larger one.
-  p.value = p.cut ? -(above ? high : low) * adv : -ratio * adv;
-  p.slope = p.cut ? 0.0f : -adv * ratio;
+  p.value = -(p.cut ? (above ? c.high : c.low) : ratio) * (double)adv;
+  p.slope = p.cut ? 0.0f : (float)-ratio * adv;
   p.kl = 0.0f;
   if (t.has_ref) {
     const float d = t.ref_lp - lp;
@@ -113,8 +118,8 @@ __device__ __forceinline__ PolicyTerm policy_term(float lp, const PolicyToken& t
     } else {
       p.kl = expf(d) - d - 1.0f;
     }
-    p.value = fmaf(c.kl_coef, p.kl, p.value);
-    p.slope = fmaf(-c.kl_coef, d + p.kl, p.slope);
+    p.value += c.kl_coef * (double)p.kl;
+    p.slope = fmaf(-(float)c.kl_coef, d + p.kl, p.slope);
   }
   return p;
 }

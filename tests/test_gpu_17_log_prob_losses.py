@@ -451,6 +451,20 @@ def test_policy_loss(otf, n, mask, has_ref, kl):
     close(grad.cpu(), 3 * want, 3 * slope_off + 6 * U * 3 * want.abs(), "gradient")
 
 
+@pytest.mark.parametrize("n", [500, 40001])
+def test_policy_loss_of_cancelling_terms(otf, n):
+    """The mean of terms of both signs, clipped ones among them, that nearly cancel: it is exact to its own size."""
+    lp, old, adv, _, _ = policy_inputs(n, None, False, n + 1)
+    old[-1], lp[-1], adv[-1] = -1.0, -1.0, 0.0
+    total = ref_policy(lp.double(), old, adv, None, None, 0.2, 0.28, 0.0)[0] * n
+    adv[-1] = total  # its ratio is 1
+    want, _, share = ref_policy(lp.double(), old, adv, None, None, 0.2, 0.28, 0.0)
+    assert abs(want) < 1e-5 and share > 0.1
+    loss = otf.losses.policy_loss(*[a.cuda() for a in (lp, old, adv)], clip_low=0.2, clip_high=0.28)[0]
+    # the result's half step, and per term the few 2^-53 of its exponential
+    close(loss.cpu(), want, U * want.abs() + 8 * 2.0 ** -53 * adv.abs().sum() / n * 1.28)
+
+
 def test_policy_borders(otf):
     """At the border itself a ratio is not clipped; beyond it on the other side of the advantage neither."""
     one = torch.zeros(5, device="cuda")
