@@ -3,7 +3,8 @@
 Compiles every ``csrc/*.cu`` for sm_100a with nvcc (in parallel, each object
 rebuilt only when its source or a header changed) and links them into
 ``opencl_tf/libb2ocl.so``, the C-ABI library declared in
-``include/b2_opencl_tf.h``.  Usage::
+``include/b2_opencl_tf.h``; and compiles ``torch_binding/*.cpp``, torch's side
+of some of its entries, into extension modules of the package with g++.  Usage::
 
     python opencl-tensorflow_b200/build.py [--force] [--verbose-ptxas]
 """
@@ -15,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -23,6 +25,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 OBJ = PKG / "_build"
 LIB = PKG / "opencl_tf" / "libb2ocl.so"
+BINDING = PKG / "torch_binding"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
@@ -54,11 +57,36 @@ def _compile(src: Path, force: bool, ptxas_v: bool) -> tuple[Path, str]:
     return obj, out.stderr if ptxas_v else ""
 
 
+def _compile_binding(src: Path, force: bool) -> Path:
+    """``opencl_tf/_<stem>.so`` from ``torch_binding/<stem>.cpp``."""
+    out = PKG / "opencl_tf" / f"_{src.stem}.so"
+    newest = max(p.stat().st_mtime for p in (src, INCLUDE / "b2_opencl_tf.h"))
+    if not force and out.exists() and out.stat().st_mtime >= newest:
+        return out
+    import torch
+    from torch.utils import cpp_extension
+    cuda = Path(nvcc()).resolve().parent.parent
+    includes = [a for p in cpp_extension.include_paths() for a in ("-isystem", p)]
+    libs = [a for p in cpp_extension.library_paths() for a in ("-L", p)]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-DTORCH_EXTENSION_NAME=_{src.stem}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *includes, "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-I", str(INCLUDE), str(src), "-o", str(out), *libs, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+           "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    return out
+
+
 def build(force: bool = False, ptxas_v: bool = False, quiet: bool = True) -> Path:
     OBJ.mkdir(exist_ok=True)
     srcs = sorted(CSRC.glob("*.cu"))
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        bindings = [ex.submit(_compile_binding, s, force) for s in sorted(BINDING.glob("*.cpp"))]
         results = list(ex.map(lambda s: _compile(s, force, ptxas_v), srcs))
+        for b in bindings:
+            b.result()
     objs = [r[0] for r in results]
     if ptxas_v and not quiet:
         for _, log in results:

@@ -28,7 +28,6 @@ import types
 from pathlib import Path
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import errors
 
@@ -40,6 +39,14 @@ if not _LIB_PATH.exists():
         f"libb2ocl.so not found at {_LIB_PATH}.\n"
         "Build it first:\n"
         "    python opencl-tensorflow_b200/build.py")
+
+try:
+    from . import _class_scores
+except ImportError as e:
+    raise ImportError(
+        f"opencl_tf/_class_scores.so cannot be loaded ({e}).\n"
+        "Build it first:\n"
+        "    python opencl-tensorflow_b200/build.py") from e
 
 _lib = ctypes.CDLL(str(_LIB_PATH))
 
@@ -597,239 +604,15 @@ def _k_upsampling_bilinear2d_grad(grad_out, input_sizes, size):
 
 # ------------------------------------------- losses over rows of class scores
 #
-# A call's cost on the host counts here (a few tokens' losses take the GPU
-# microseconds): arguments are checked in one test each, with the reason looked for
-# only when it fails, and the stream is fetched as a plain handle.
+# Their argument checks, outputs and autograd nodes are compiled
+# (torch_binding/class_scores.cpp): a few tokens' losses take the GPU microseconds,
+# and a node in Python would cost the host fifty.
 
-_FLOATS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # b2_dtype_t
-_INTS = (torch.int64, torch.int32)
-_WEIGHTS = (torch.float32, torch.bool, torch.uint8)
-_F32_ONLY = (torch.float32,)
-
-
-def _on_cuda(t, what: str) -> None:
-    if not isinstance(t, torch.Tensor):
-        raise errors.InvalidArgumentError(f"{what} must be a torch tensor on a CUDA device")
-    if not t.is_cuda:
-        raise errors.InvalidArgumentError(
-            f"{what} must live on a CUDA device (this backend has no CPU path)")
-
-
-def _logits(t, what: str):
-    """(tensor, b2_logits_t) of scores [..., classes]; leading axes that fold
-    into two strides are read in place, others are copied."""
-    _on_cuda(t, what)
-    dtype = _FLOATS.get(t.dtype)
-    if dtype is None:
-        raise errors.InvalidArgumentError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
-    if t.dim() < 1 or t.shape[-1] < 1:
-        raise errors.InvalidArgumentError(f"{what} must be [..., classes] with at least one class")
-    classes = t.shape[-1]
-    if not t.is_contiguous():
-        axes = []  # (size, stride) of the leading axes, adjacent ones folded
-        for size, stride in zip(t.shape[:-1], t.stride()[:-1]):
-            if size == 1:
-                continue
-            if axes and axes[-1][1] == size * stride:
-                axes[-1] = (axes[-1][0] * size, stride)
-            else:
-                axes.append((size, stride))
-        if len(axes) <= 2 and (t.stride(-1) == 1 or classes == 1):
-            (outer, so), (inner, si) = [(1, 0)] * (2 - len(axes)) + axes
-            return t, Logits(t.data_ptr(), dtype, outer, inner, classes, so, si)
-        t = t.contiguous()
-    return t, Logits(t.data_ptr(), dtype, 1, t.numel() // classes, classes, 0, classes)
-
-
-def _refuse(t, what, shape, dev, dtypes):
-    _on_cuda(t, what)
-    if t.dtype not in dtypes:
-        names = ", ".join(str(d).removeprefix("torch.") for d in dtypes)
-        raise errors.InvalidArgumentError(f"{what} must be {names}, got {t.dtype}")
-    if t.shape != shape:
-        raise errors.InvalidArgumentError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    raise errors.InvalidArgumentError(f"{what} must live on cuda:{dev}, got {t.device}")
-
-
-def _same(t, what: str, shape, dev: int, dtypes) -> torch.Tensor:
-    if not (isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype in dtypes and t.shape == shape):
-        _refuse(t, what, shape, dev, dtypes)
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _opt_same(t, what, shape, dev, dtypes):
-    return None if t is None else _same(t, what, shape, dev, dtypes)
-
-
-def _scalar(t, what, dev):
-    if t is None:
-        return None
-    if not (isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype == torch.float32 and t.numel() == 1):
-        _on_cuda(t, what)
-        raise errors.InvalidArgumentError(f"{what} must be a float32 scalar on cuda:{dev}")
-    return t
-
-
-def _opt(t):
-    return None if t is None else t.data_ptr()
-
-
-def _size(t):
-    return 0 if t is None else t.element_size()
-
-
-def _f32(like, shape):
-    return like.new_empty(shape, dtype=torch.float32)
-
-
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _call(dev: int, entry, *args) -> None:
-    """Calls a C entry on device ``dev`` and torch's current stream of it."""
-    if torch.cuda.current_device() == dev:
-        rc = entry(_raw_stream(dev), *args)
-    else:
-        with torch.cuda.device(dev):
-            rc = entry(_raw_stream(dev), *args)
-    if rc:
-        _check(rc)
-
-
-def _k_token_log_probs(logits, targets, with_stats=False):
-    x, v = _logits(logits, "logits")
-    dev, lead = x.get_device(), x.shape[:-1]
-    t = _same(targets, "targets", lead, dev, _INTS)
-    out = _f32(x, lead)
-    stats = _f32(x, (*lead, 2)) if with_stats else None
-    _call(dev, _lib.b2_token_log_probs, ctypes.byref(v), t.data_ptr(), t.element_size(), out.data_ptr(), _opt(stats))
-    return (out, stats) if with_stats else out
-
-
-def _k_token_log_probs_grad(grad_log_probs, logits, targets, row_stats):
-    x, v = _logits(logits, "logits")
-    dev, lead = x.get_device(), x.shape[:-1]
-    t = _same(targets, "targets", lead, dev, _INTS)
-    g = _same(grad_log_probs, "grad_log_probs", lead, dev, _F32_ONLY)
-    out = x.new_empty(x.shape)
-    _call(dev, _lib.b2_token_log_probs_grad, ctypes.byref(v), t.data_ptr(), t.element_size(), row_stats.data_ptr(),
-          g.data_ptr(), out.data_ptr())
-    return out
-
-
-def _teacher(x, dev, lead, teacher_ids, teacher_logits, weights):
-    if not isinstance(teacher_ids, torch.Tensor) or teacher_ids.dim() != x.dim():
-        raise errors.InvalidArgumentError("teacher_ids must be [..., entries] with the leading axes of logits")
-    ids = _same(teacher_ids, "teacher_ids", (*lead, teacher_ids.shape[-1]), dev, _INTS)
-    y = _same(teacher_logits, "teacher_logits", ids.shape, dev, _FLOATS)
-    return ids, y, _opt_same(weights, "weights", lead, dev, _WEIGHTS)
-
-
-def _k_distillation_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0, with_stats=False,
-                         with_grad=False, grad_loss=None):
-    x, v = _logits(logits, "logits")
-    dev, lead = x.get_device(), x.shape[:-1]
-    ids, y, w = _teacher(x, dev, lead, teacher_ids, teacher_logits, weights)
-    gl = _scalar(grad_loss, "grad_loss", dev)
-    loss = _f32(x, ())
-    stats = _f32(x, 4 * (v.outer * v.inner) + 2)  # the call's workspace, too
-    grad = x.new_empty(x.shape) if with_grad else None
-    _call(dev, _lib.b2_distillation_loss, ctypes.byref(v), ids.data_ptr(), ids.element_size(), y.data_ptr(),
-          _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w), float(temperature), loss.data_ptr(),
-          stats.data_ptr(), _opt(gl), _opt(grad))
-    return (loss, stats) if with_stats else (loss, grad) if with_grad else loss
-
-
-def _k_distillation_loss_grad(logits, teacher_ids, teacher_logits, weights, temperature, row_stats, grad_loss):
-    x, v = _logits(logits, "logits")
-    dev, lead = x.get_device(), x.shape[:-1]
-    ids, y, w = _teacher(x, dev, lead, teacher_ids, teacher_logits, weights)
-    gl = _scalar(grad_loss, "grad_loss", dev)
-    out = x.new_empty(x.shape)
-    _call(dev, _lib.b2_distillation_loss_grad, ctypes.byref(v), ids.data_ptr(), ids.element_size(), y.data_ptr(),
-          _FLOATS[y.dtype], ids.shape[-1], _opt(w), _size(w), float(temperature), row_stats.data_ptr(),
-          gl.data_ptr(), out.data_ptr())
-    return out
-
-
-def _log_probs(t, what="log_probs"):
-    _on_cuda(t, what)
-    if t.dtype != torch.float32:
-        raise errors.InvalidArgumentError(f"{what} must be float32, got {t.dtype}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _k_preference_loss(log_probs, offsets, ref_log_probs=None, mask=None, beta=0.1, label_smoothing=0.0):
-    """-> loss, rewards [2 * pairs], slopes [2 * pairs]"""
-    lp = _log_probs(log_probs)
-    dev, shape = lp.get_device(), lp.shape
-    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 3 or offsets.numel() % 2 == 0:
-        raise errors.InvalidArgumentError("offsets must have 2 * pairs + 1 elements, pairs >= 1")
-    off = _same(offsets, "offsets", offsets.shape, dev, _INTS)
-    ref = _opt_same(ref_log_probs, "ref_log_probs", shape, dev, _F32_ONLY)
-    w = _opt_same(mask, "mask", shape, dev, _WEIGHTS)
-    sequences = off.numel() - 1
-    loss, rewards, slopes = lp.new_empty(()), lp.new_empty(sequences), lp.new_empty(sequences)
-    _call(dev, _lib.b2_preference_loss, lp.data_ptr(), _opt(ref), _opt(w), _size(w), lp.numel(), off.data_ptr(),
-          off.element_size(), sequences // 2, float(beta), float(label_smoothing), loss.data_ptr(),
-          rewards.data_ptr(), slopes.data_ptr())
-    return loss, rewards, slopes
-
-
-def _k_preference_loss_grad(grad_loss, slopes, offsets, mask, shape):
-    dev = slopes.get_device()
-    gl = _scalar(grad_loss, "grad_loss", dev)
-    off = offsets if offsets.is_contiguous() else offsets.contiguous()
-    w = _opt_same(mask, "mask", shape, dev, _WEIGHTS)
-    out = slopes.new_empty(shape)
-    _call(dev, _lib.b2_preference_loss_grad, gl.data_ptr(), slopes.data_ptr(), _opt(w), _size(w), out.numel(),
-          off.data_ptr(), off.element_size(), slopes.numel() // 2, out.data_ptr())
-    return out
-
-
-def _policy_inputs(shape, dev, old_log_probs, advantages, ref_log_probs, mask):
-    return (_same(old_log_probs, "old_log_probs", shape, dev, _F32_ONLY),
-            _same(advantages, "advantages", shape, dev, _F32_ONLY),
-            _opt_same(ref_log_probs, "ref_log_probs", shape, dev, _F32_ONLY),
-            _opt_same(mask, "mask", shape, dev, _WEIGHTS))
-
-
-def _k_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs=None, mask=None, clip_low=0.2, clip_high=0.2,
-                   kl_coef=0.0, with_slopes=False):
-    """-> loss, stats (mean KL, clipped share, 1 / sum of the weights), slopes or None"""
-    lp = _log_probs(log_probs)
-    dev = lp.get_device()
-    old, adv, ref, w = _policy_inputs(lp.shape, dev, old_log_probs, advantages, ref_log_probs, mask)
-    loss, stats = lp.new_empty(()), lp.new_empty(3)
-    slopes = lp.new_empty(lp.shape) if with_slopes else None
-    _call(dev, _lib.b2_policy_loss, lp.data_ptr(), old.data_ptr(), adv.data_ptr(), _opt(ref), _opt(w), _size(w),
-          lp.numel(), float(clip_low), float(clip_high), float(kl_coef), loss.data_ptr(), stats.data_ptr(),
-          _opt(slopes))
-    return loss, stats, slopes
-
-
-def _k_policy_loss_grad(grad_loss, stats, slopes):
-    dev = slopes.get_device()
-    gl = _scalar(grad_loss, "grad_loss", dev)
-    out = slopes.new_empty(slopes.shape)
-    _call(dev, _lib.b2_policy_loss_grad, gl.data_ptr(), stats.data_ptr(), slopes.data_ptr(), out.numel(),
-          out.data_ptr())
-    return out
-
-
-def _k_policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs=None, mask=None, clip_low=0.2,
-                             clip_high=0.2, kl_coef=0.0, grad_loss=None):
-    """-> loss, stats (mean KL, clipped share), grad_logits"""
-    x, v = _logits(logits, "logits")
-    dev, lead = x.get_device(), x.shape[:-1]
-    t = _same(targets, "targets", lead, dev, _INTS)
-    old, adv, ref, w = _policy_inputs(lead, dev, old_log_probs, advantages, ref_log_probs, mask)
-    gl = _scalar(grad_loss, "grad_loss", dev)
-    loss, stats, grad = _f32(x, ()), _f32(x, 2), x.new_empty(x.shape)
-    _call(dev, _lib.b2_policy_loss_with_grad, ctypes.byref(v), t.data_ptr(), t.element_size(), old.data_ptr(),
-          adv.data_ptr(), _opt(ref), _opt(w), _size(w), float(clip_low), float(clip_high), float(kl_coef), _opt(gl),
-          loss.data_ptr(), stats.data_ptr(), grad.data_ptr())
-    return loss, stats, grad
+_CLASS_SCORE_ENTRIES = ("b2_token_log_probs", "b2_token_log_probs_grad", "b2_distillation_loss",
+                        "b2_distillation_loss_grad", "b2_preference_loss", "b2_preference_loss_grad", "b2_policy_loss",
+                        "b2_policy_loss_grad", "b2_policy_loss_with_grad")
+_class_scores.bind([ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in _CLASS_SCORE_ENTRIES],
+                   errors.InvalidArgumentError, _check)
 
 
 # ------------------------------------------------------- gradient registry
@@ -898,88 +681,6 @@ def _apply(op_type: str, kernel, inputs, attrs, nondiff=()):
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
         return _OpNode.apply(op_type, attrs, kernel, tuple(nondiff), *inputs)
     return kernel(*inputs, **attrs)
-
-
-# The losses' gradients need more than an op's inputs and outputs (the rows'
-# softmax statistics, the slopes of sequences and tokens), so each is an
-# autograd node of its own instead of a registered gradient function.  They are
-# differentiable once: a backward pass that is itself recorded (create_graph) gets
-# an error node, any other one goes straight to the kernel.
-
-def _once(backward):
-    recorded = once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return recorded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-
-    return staticmethod(run)
-
-
-class _TokenLogProbsNode(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, targets):
-        out, stats = _k_token_log_probs(logits, targets, with_stats=True)
-        ctx.save_for_backward(logits, targets, stats)
-        return out
-
-    @_once
-    def backward(ctx, grad):
-        logits, targets, stats = ctx.saved_tensors
-        return _k_token_log_probs_grad(grad, logits, targets, stats), None
-
-
-class _DistillationNode(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, teacher_ids, teacher_logits, weights, temperature):
-        loss, stats = _k_distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature, with_stats=True)
-        ctx.save_for_backward(logits, teacher_ids, teacher_logits, weights, stats)
-        ctx.temperature = temperature
-        return loss
-
-    @_once
-    def backward(ctx, grad):
-        logits, ids, y, weights, stats = ctx.saved_tensors
-        return _k_distillation_loss_grad(logits, ids, y, weights, ctx.temperature, stats, grad), None, None, None, None
-
-
-class _PreferenceNode(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, log_probs, offsets, ref_log_probs, mask, beta, label_smoothing):
-        loss, rewards, slopes = _k_preference_loss(log_probs, offsets, ref_log_probs, mask, beta, label_smoothing)
-        ctx.save_for_backward(offsets, mask, slopes)
-        ctx.shape = log_probs.shape
-        ctx.mark_non_differentiable(rewards)
-        ctx.set_materialize_grads(False)
-        return loss, rewards
-
-    @_once
-    def backward(ctx, grad, _grad_rewards):
-        if grad is None:
-            return (None,) * 6
-        offsets, mask, slopes = ctx.saved_tensors
-        return _k_preference_loss_grad(grad, slopes, offsets, mask, ctx.shape), None, None, None, None, None
-
-
-class _PolicyNode(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low, clip_high, kl_coef):
-        loss, stats, slopes = _k_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low,
-                                             clip_high, kl_coef, with_slopes=True)
-        ctx.save_for_backward(stats, slopes)
-        ctx.mark_non_differentiable(stats)
-        ctx.set_materialize_grads(False)
-        return loss, stats
-
-    @_once
-    def backward(ctx, grad, _grad_stats):
-        if grad is None:
-            return (None,) * 8
-        stats, slopes = ctx.saved_tensors
-        return _k_policy_loss_grad(grad, stats, slopes), None, None, None, None, None, None, None
-
-
-def _differentiable(t) -> bool:
-    return isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled()
 
 
 # --------------------------------------------------------------- raw_ops
@@ -1121,40 +822,31 @@ def _mk_step_ops():
         return _k_mse_loss_grad(y_pred, y_true, grad_loss)
 
     def opencl_token_log_probs(logits, targets):
-        if _differentiable(logits):
-            return _TokenLogProbsNode.apply(logits, targets)
-        return _k_token_log_probs(logits, targets)
+        return _class_scores.token_log_probs(logits, targets)
 
     def opencl_distillation_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0):
-        if _differentiable(logits):
-            return _DistillationNode.apply(logits, teacher_ids, teacher_logits, weights, float(temperature))
-        return _k_distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature)
+        return _class_scores.distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature)
 
     def opencl_distillation_loss_with_grad(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0,
                                            grad_loss=None):
-        return _k_distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature, with_grad=True,
-                                    grad_loss=grad_loss)
+        return _class_scores.distillation_loss_with_grad(logits, teacher_ids, teacher_logits, weights, temperature,
+                                                         grad_loss)
 
     def opencl_preference_loss(log_probs, offsets, ref_log_probs=None, mask=None, beta=0.1, label_smoothing=0.0):
         """-> loss, rewards of the 2 * pairs sequences"""
-        if _differentiable(log_probs):
-            return _PreferenceNode.apply(log_probs, offsets, ref_log_probs, mask, float(beta), float(label_smoothing))
-        return _k_preference_loss(log_probs, offsets, ref_log_probs, mask, beta, label_smoothing)[:2]
+        return _class_scores.preference_loss(log_probs, offsets, ref_log_probs, mask, beta, label_smoothing)
 
     def opencl_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs=None, mask=None, clip_low=0.2,
                            clip_high=0.2, kl_coef=0.0):
         """-> loss, stats (mean KL, clipped share, 1 / sum of the weights)"""
-        if _differentiable(log_probs):
-            return _PolicyNode.apply(log_probs, old_log_probs, advantages, ref_log_probs, mask, float(clip_low),
-                                     float(clip_high), float(kl_coef))
-        return _k_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low, clip_high,
-                              kl_coef)[:2]
+        return _class_scores.policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low,
+                                         clip_high, kl_coef)
 
     def opencl_policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs=None, mask=None,
                                      clip_low=0.2, clip_high=0.2, kl_coef=0.0, grad_loss=None):
         """-> loss, stats (mean KL, clipped share), grad_logits"""
-        return _k_policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs, mask, clip_low,
-                                        clip_high, kl_coef, grad_loss)
+        return _class_scores.policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs, mask,
+                                                   clip_low, clip_high, kl_coef, grad_loss)
 
     for k, v in list(locals().items()):
         if k.startswith("opencl_"):
