@@ -401,7 +401,8 @@ __device__ __forceinline__ int filter_word(int id, int filter_words) { return (i
 
 // A row's lanes lay out its teacher: softmax over the entries whose class
 // lies in the row and whose logit is not -inf.  Returns false when there is none.
-template <class T, int kLanes>
+// Without kScores the row's scores of the entries are left to load_scores.
+template <class T, int kLanes, bool kScores>
 __device__ __forceinline__ bool load_teacher(const RowArgs& A, int64_t r, const T* row, int lane, const Teacher& t,
                                              float* ymax, float* sum_q) {
   const int64_t base = r * A.top;
@@ -416,7 +417,7 @@ __device__ __forceinline__ bool load_teacher(const RowArgs& A, int64_t r, const 
     const float y = real ? y0 : -INFINITY;
     t.ids[k] = real ? (int)id : -1;
     t.q[k] = y;
-    t.x[k] = real ? Pack<T>::one(row[id]) : 0.0f;
+    if (kScores) t.x[k] = real ? Pack<T>::one(row[id]) : 0.0f;
     mx = fmaxf(mx, y);
     nan |= y != y;
   }
@@ -442,6 +443,16 @@ __device__ __forceinline__ bool load_teacher(const RowArgs& A, int64_t r, const 
   *ymax = mx;
   *sum_q = sum;
   return true;
+}
+
+// Where the row has just been added up, they are near: read ahead of it they cost
+// 131072 x 2000 bf16, 64 entries, 85 us.
+template <class T, int kLanes>
+__device__ __forceinline__ void load_scores(const RowArgs& A, const T* row, int lane, const Teacher& t) {
+  for (int k = lane; k < A.top; k += kLanes) {
+    const int id = t.ids[k];
+    t.x[k] = id >= 0 ? Pack<T>::one(row[id]) : 0.0f;
+  }
 }
 
 // Sum of q over the entries of the class of entry k, added in the entries'
@@ -614,7 +625,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kS
   bool real = true;
   if (helper) {
     if (kMode == kDistill) {
-      real = load_teacher<T, 32>(A, r, row, lane, teacher, &ymax, &sum_q);
+      real = load_teacher<T, 32, true>(A, r, row, lane, teacher, &ymax, &sum_q);
       if (lane == 0) {
         if (kGrad) factor_s = A.temperature * w * unit_share(A);
         real_s = real;
@@ -697,13 +708,16 @@ template <int kGroup>
 constexpr int cta_threads() {
   return kGroup <= 32 ? 256 : kGroup;
 }
-template <bool kA, bool kB>
+// On an SM.  More writing streams are slower (gradient of 65536 x 4000 bf16: 182 us,
+// with 1536 threads 227), and a teacher's row takes registers (its loss and gradient,
+// 64 entries: 318 us, with 1024 threads 378).
+template <int kMode, bool kA, bool kB>
 constexpr int resident_threads() {
-  return kB ? 1024 : 1536;  // on an SM: more writing streams are slower (65536 x 4000 bf16: 182 us, 1536 threads 227)
+  return !kB ? 1536 : kMode == kDistill && kA ? 768 : 1024;
 }
 
 template <class T, int kMode, int kGroup, bool kA, bool kB>
-__global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kA, kB>() / cta_threads<kGroup>())
+__global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kMode, kA, kB>() / cta_threads<kGroup>())
     rows_kernel(const __grid_constant__ RowArgs A) {
   constexpr int kThreads = cta_threads<kGroup>(), kGroups = kThreads / kGroup, kWarps = kThreads / 32;
   constexpr int kLanes = kGroup < 32 ? kGroup : 32;
@@ -751,7 +765,7 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kA, kB
       if (leader && b.real) b.x_target = Pack<T>::one(row[h.target]);
     } else if (leader) {
       __syncwarp(lanes_mask<kLanes>());  // the row that had this buffer is done with it
-      b.real = load_teacher<T, kLanes>(A, i, row, lane, teacher_of(buf), &b.ymax, &b.sum_q);
+      b.real = load_teacher<T, kLanes, !kA>(A, i, row, lane, teacher_of(buf), &b.ymax, &b.sum_q);
       if (kCta && lane == 0) real_s[buf] = b.real;
     }
     if (!kA) {
@@ -783,6 +797,7 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kA, kB
         factor = -now.up;
       } else if (kMode == kDistill) {
         if (kA && leader) {
+          if (row.real) load_scores<T, kLanes>(A, row_at<T>(A, r), lane, teacher_of(buf));
           const double loss =
               row.real ? distill_row<kLanes>(A, r, lane, teacher_of(buf), row.st, row.ymax, row.sum_q, now.w) : 0.0;
           if (lane == 0) A.row_out[r] = loss;
@@ -876,22 +891,30 @@ int launch_groups(cudaStream_t s, const RowArgs& a, int per_sm, const DeviceInfo
 constexpr int64_t kLongRow = 16 * 1024;     // bytes; shorter rows end too often for long_kernel
 constexpr int64_t kSliceBytes = 140 * 1024;  // of a row that is read twice, see long_kernel
 constexpr int64_t kWideSlice = 96 * 1024;    // from here 16 warps and not 8
+// Bytes of a teacher (256 entries) that a row of rows_kernel may have.  With more
+// its warp is what the CTA waits for: 65536 x 4000 bf16, 1024 entries, takes 6.0 ms
+// there and 2.5 as CTAs with a warp for it.
+constexpr int kFewEntries = 4096;
 
 // kA: pass 1 (statistics and loss), kB: pass 2 (gradient).
 template <class T, int kMode, bool kA, bool kB>
 int launch_rows_as(cudaStream_t s, RowArgs a, const DeviceInfo* d, const char* what) {
   const int64_t sms = d->sm_count;
-  constexpr int resident = resident_threads<kA, kB>();
+  constexpr int resident = resident_threads<kMode, kA, kB>();
   if (kMode == kDistill) {
+    // 32 bits an entry, so that few entries look repeated without being it: 8192 x 32000
+    // bf16, 1024 entries, takes 534 us, with 4 bits an entry 1192.
     a.filter_words = 4;
-    while (a.filter_words < 128 && a.filter_words * 4 < a.top) a.filter_words *= 2;
+    while (a.filter_words < (a.top > 256 ? 512 : 128) && a.filter_words < a.top) a.filter_words *= 2;
     a.teacher_bytes = (int)ceil_div(4 * (2 * a.filter_words + 3 * a.top), 16) * 16;
   }
   const bool fill8 = a.rows * 8 >= sms * resident, fill32 = a.rows * 32 >= sms * resident;
   // Forward alone: lanes of a warp keep up to rows of 16384 values, when there are twice as many as run at once.
-  if (!kB && a.classes > 4096 && a.classes <= 16384 && a.rows * 32 >= 2 * sms * resident && a.teacher_bytes <= 4096)
+  if (!kB && a.classes > 4096 && a.classes <= 16384 && a.rows * 32 >= 2 * sms * resident &&
+      a.teacher_bytes <= kFewEntries)
     return launch_groups<T, kMode, 32, kA, kB>(s, a, resident / 256, d, what);
-  if (a.classes >= kLongRow / (int64_t)sizeof(T) || (a.rows <= 2 * sms && a.classes >= 4096)) {
+  if (a.classes >= kLongRow / (int64_t)sizeof(T) || (a.rows <= 2 * sms && a.classes >= 4096) ||
+      a.teacher_bytes > kFewEntries) {
     // A cluster for a row whose slice L2 would not keep, and, for few rows, while
     // there are fewer CTAs than SMs and a slice keeps 2048 values.
     auto slice_of = [&](int ctas) { return ceil_div(ceil_div((int64_t)a.classes, ctas), 8) * 8; };
@@ -909,9 +932,9 @@ int launch_rows_as(cudaStream_t s, RowArgs a, const DeviceInfo* d, const char* w
   }
   // As few threads a row as keep the SMs full; where each writes, 8 lanes' 128
   // bytes a row are too small a piece of longer rows.
-  if (a.classes <= (!kB ? 4096 : kA ? 2048 : 1024) && fill8 && a.teacher_bytes <= 512)
+  if (a.classes <= (!kB ? 4096 : kA ? 2048 : 1024) && fill8 && a.teacher_bytes <= 640)
     return launch_groups<T, kMode, 8, kA, kB>(s, a, resident / 256, d, what);
-  if ((a.classes <= 1024 || (fill32 && a.classes <= 8192)) && a.teacher_bytes <= 4096)
+  if ((a.classes <= 1024 || (fill32 && a.classes <= 8192)) && a.teacher_bytes <= kFewEntries)
     return launch_groups<T, kMode, 32, kA, kB>(s, a, resident / 256, d, what);
   return launch_groups<T, kMode, 256, kA, kB>(s, a, resident / 256, d, what);
 }

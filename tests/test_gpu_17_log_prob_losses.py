@@ -259,7 +259,7 @@ def teacher(x, k, seed, dtype=torch.float32):
 
 
 DISTILL = [(1, 1, 1), (4, 2, 3), (33, 70, 8), (5, 1000, 1024), (7, 1025, 1), (3, 5000, 64), (1, 32003, 100),
-           (300, 2050, 17), (2, 131075, 128)]
+           (300, 2050, 17), (2, 131075, 128), (200, 4003, 600), (30, 129, 257)]
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
