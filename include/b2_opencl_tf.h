@@ -434,7 +434,8 @@ int b2_token_log_probs_grad(b2_stream_t stream, const b2_logits_t* logits,
  *                * (P[r, j] - sum_{k: id[r,k] == j} q[r,k])
  * grad_loss: a device float, or null for 1.  row_stats: 4 * rows + 2 floats,
  * 8-byte aligned, for b2_distillation_loss_grad (each row's statistics as above,
- * the sum of the weights and room for the rows' losses), or null. */
+ * the sum infinite for a row without entries; the sum of the weights; room for
+ * the rows' losses), or null. */
 int b2_distillation_loss(b2_stream_t stream, const b2_logits_t* logits,
                          const void* teacher_ids, int id_bytes,
                          const void* teacher_logits, int teacher_dtype,

@@ -121,7 +121,8 @@ __device__ __forceinline__ double sequence_part(const PreferenceArgs& A, int64_t
 }
 
 // One CTA per sequence: rewards[i] = beta sum_n w_n (lp_n - ref_n).
-__global__ void __launch_bounds__(kTokenThreads) sequence_sum_kernel(const PreferenceArgs A, double* __restrict__ sums) {
+__global__ void __launch_bounds__(kTokenThreads)
+    sequence_sum_kernel(const PreferenceArgs A, double* __restrict__ sums) {
   __shared__ double part[kTokenThreads / 32];
   const int64_t i = blockIdx.x;
   const double v = warp_sum(sequence_part(A, i, threadIdx.x, kTokenThreads));
@@ -228,8 +229,8 @@ constexpr int kPolicySums = 4;  // loss, kl, clipped, weights
 // (3.9 us) and at a million (11.4 us with the second launch); there a mean of terms
 // that cancel to 1e-3 was 7e-7 off with ratios in 32.  Loads that do not wait for
 // the token's weight, and four tokens a turn, are no faster at a million.
-__device__ __forceinline__ void policy_part(const PolicyArgs& A, int64_t first, int64_t step, float* __restrict__ slopes,
-                                            double* v) {
+__device__ __forceinline__ void policy_part(const PolicyArgs& A, int64_t first, int64_t step,
+                                            float* __restrict__ slopes, double* v) {
   const bool has_ref = A.ref_lp != nullptr;
   for (int64_t n = first; n < A.tokens; n += step) {
     const float w = weight_at(A.mask, A.mask_bytes, n);
@@ -261,7 +262,8 @@ __device__ __forceinline__ void store_means(const double* v, float* __restrict__
 constexpr int kFewPolicyTokens = 8 * kSumCtas * kSumThreads;
 
 __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
-    few_policy_kernel(const PolicyArgs A, float* __restrict__ slopes, float* __restrict__ loss, float* __restrict__ stats) {
+    few_policy_kernel(const PolicyArgs A, float* __restrict__ slopes, float* __restrict__ loss,
+                      float* __restrict__ stats) {
   double v[kPolicySums] = {};
   policy_part(A, (int64_t)blockIdx.x * kSumThreads + threadIdx.x, kSumCtas * kSumThreads, slopes, v);
   cluster_sum<kPolicySums>(v);
@@ -404,8 +406,8 @@ static int distill_args(const b2_logits_t* logits, const void* teacher_ids, int 
   B2_RETURN_IF_ERROR(index_ok(id_bytes, what, "teacher_ids"));
   B2_RETURN_IF_ERROR(weight_ok(weights, weight_bytes, what));
   B2_REQUIRE(a->rows > 0, "%s: the mean over no rows is undefined", what);
-  B2_REQUIRE(top >= 1 && top <= kMaxTop, "%s: the teacher's entries per row must be in [1, %d], got %lld", what, kMaxTop,
-             (long long)top);
+  B2_REQUIRE(top >= 1 && top <= kMaxTop, "%s: the teacher's entries per row must be in [1, %d], got %lld", what,
+             kMaxTop, (long long)top);
   B2_REQUIRE(teacher_dtype == B2_FLOAT32 || teacher_dtype == B2_FLOAT16 || teacher_dtype == B2_BFLOAT16,
              "%s: teacher_logits must be float32, float16 or bfloat16", what);
   B2_REQUIRE(temperature >= 1e-30 && temperature <= 1e30, "%s: temperature must be in [1e-30, 1e30]", what);
@@ -543,7 +545,8 @@ int b2_policy_loss(b2_stream_t stream, const float* log_probs, const float* old_
   clear_error();
   const char* what = "policy_loss";
   B2_RETURN_IF_ERROR(policy_ok(tokens, mask, mask_bytes, clip_low, clip_high, kl_coef, what));
-  B2_REQUIRE(log_probs != nullptr && old_log_probs != nullptr && advantages != nullptr && loss != nullptr && stats != nullptr,
+  B2_REQUIRE(log_probs != nullptr && old_log_probs != nullptr && advantages != nullptr && loss != nullptr &&
+                 stats != nullptr,
              "policy_loss: null pointer");
   const DeviceInfo* d = nullptr;
   B2_RETURN_IF_ERROR(device_info(&d));
@@ -587,8 +590,8 @@ int b2_policy_loss_with_grad(b2_stream_t stream, const b2_logits_t* logits, cons
   B2_RETURN_IF_ERROR(row_args(logits, what, &a));
   B2_RETURN_IF_ERROR(index_ok(target_bytes, what, "targets"));
   B2_RETURN_IF_ERROR(policy_ok(a.rows, mask, mask_bytes, clip_low, clip_high, kl_coef, what));
-  B2_REQUIRE(targets != nullptr && old_log_probs != nullptr && advantages != nullptr && loss != nullptr && stats != nullptr &&
-                 grad_logits != nullptr,
+  B2_REQUIRE(targets != nullptr && old_log_probs != nullptr && advantages != nullptr && loss != nullptr &&
+                 stats != nullptr && grad_logits != nullptr,
              "policy_loss_with_grad: null pointer");
   const DeviceInfo* d = nullptr;
   B2_RETURN_IF_ERROR(device_info(&d));

@@ -206,7 +206,9 @@ void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 float* floats(const Tensor& t) { return static_cast<float*>(data(t)); }
 int width(const Tensor& t) { return t.defined() ? static_cast<int>(t.element_size()) : 0; }
 
-Tensor new_f32(const Tensor& like, c10::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
+Tensor new_f32(const Tensor& like, c10::IntArrayRef shape) {
+  return at::empty(shape, like.options().dtype(at::kFloat));
+}
 Tensor new_dense(const Tensor& like) { return at::empty(like.sizes(), like.options()); }
 
 bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
@@ -248,8 +250,8 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
       const Rows x = rows_of(logits);
       const Tensor g = grads[0].contiguous();
       out = new_dense(logits);
-      call(true, logits, entries.token_log_probs_grad, &x, targets.data_ptr(), width(targets), floats(saved[2]), floats(g),
-           out.data_ptr());
+      call(true, logits, entries.token_log_probs_grad, &x, targets.data_ptr(), width(targets), floats(saved[2]),
+           floats(g), out.data_ptr());
     }
     return {once(out, logits), Tensor()};
   }
@@ -286,8 +288,8 @@ struct Distillation : torch::autograd::Function<Distillation> {
     const Rows x = rows_of(logits);
     Tensor loss = new_f32(logits, {});
     call(false, logits, entries.distillation_loss, &x, t.ids.data_ptr(), width(t.ids), t.y.data_ptr(),
-         static_cast<int>(dtype_of(t.y)), t.ids.size(-1), data(t.weights), width(t.weights), t.temperature, floats(loss),
-         floats(stats), floats(grad_loss), data(grad));
+         static_cast<int>(dtype_of(t.y)), t.ids.size(-1), data(t.weights), width(t.weights), t.temperature,
+         floats(loss), floats(stats), floats(grad_loss), data(grad));
     return loss;
   }
   static Tensor new_stats(const Tensor& logits) { return new_f32(logits, {4 * rows_in(logits) + 2}); }
