@@ -323,8 +323,17 @@ __device__ __forceinline__ uint4 scaled_vector(const uint4& u, float m, float c,
   return Pack<T>::pack(f);
 }
 
+// A vector's last read.  kAgain: it was read before, in this launch: marked as
+// streamed it leaves room for others (131072 x 2000 bf16, loss and gradient: 272 us,
+// unmarked 347).  Marked, a gradient alone is slower: 524288 x 500 249 us and not 203,
+// distillation's of 8192 x 32000 190 and not 172 (but 16384 x 16000 187 and not 196).
+template <bool kAgain>
+__device__ __forceinline__ uint4 load_last(const uint4* p) {
+  return kAgain ? __ldcs(p) : __ldg(p);
+}
+
 // out[j] = factor * 2^((row[j] - m) c) in the row's vectors (of which `sp` tells).
-template <class T, int kGroup>
+template <class T, int kGroup, bool kAgain>
 __device__ __forceinline__ void write_vectors(const T* __restrict__ row, T* __restrict__ out, const Span& sp, int n,
                                               int g, float m, float c, float factor) {
   const uint4* __restrict__ v = reinterpret_cast<const uint4*>(row + sp.head);
@@ -333,7 +342,7 @@ __device__ __forceinline__ void write_vectors(const T* __restrict__ row, T* __re
   for (; i + (kBatch - 1) * kGroup < sp.nvec; i += kBatch * kGroup) {
     uint4 u[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) u[k] = __ldcs(v + i + k * kGroup);
+    for (int k = 0; k < kBatch; ++k) u[k] = load_last<kAgain>(v + i + k * kGroup);
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) __stcs(w + i + k * kGroup, scaled_vector<T>(u[k], m, c, factor));
   }
@@ -341,7 +350,7 @@ __device__ __forceinline__ void write_vectors(const T* __restrict__ row, T* __re
     uint4 u[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k)
-      if (i + k * kGroup < sp.nvec) u[k] = __ldcs(v + i + k * kGroup);
+      if (i + k * kGroup < sp.nvec) u[k] = load_last<kAgain>(v + i + k * kGroup);
 #pragma unroll
     for (int k = 0; k < kBatch; ++k)
       if (i + k * kGroup < sp.nvec) __stcs(w + i + k * kGroup, scaled_vector<T>(u[k], m, c, factor));
@@ -351,14 +360,14 @@ __device__ __forceinline__ void write_vectors(const T* __restrict__ row, T* __re
 // A slice's gradient without its chosen classes.  Where row and output do not
 // lie equally far from a 16-byte border, the values of an output vector are
 // read one by one.
-template <class T, int kGroup>
+template <class T, int kGroup, bool kAgain>
 __device__ __forceinline__ void write_slice(const T* __restrict__ row, T* __restrict__ out, int n, int g, float m,
                                             float c, float factor) {
   constexpr int N = Pack<T>::n;
   const Span sp = span_of(out, n);
   write_edges(row, out, sp, n, g, m, c, factor);
   if (same_border<T>(row, out)) {
-    write_vectors<T, kGroup>(row, out, sp, n, g, m, c, factor);
+    write_vectors<T, kGroup, kAgain>(row, out, sp, n, g, m, c, factor);
     return;
   }
   uint4* __restrict__ w = reinterpret_cast<uint4*>(out + sp.head);
@@ -693,7 +702,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kS
   const bool writes = kMode != kDistill ? target >= 0 : kStats ? real_s != 0 : st.s != INFINITY;
   if (!helper) {
     if (writes)
-      write_slice<T, kThreads>(mine, out, n, g, st.m, A.c, factor * inv_s);
+      write_slice<T, kThreads, kStats>(mine, out, n, g, st.m, A.c, factor * inv_s);
     else
       zero_slice<T, kThreads>(out, n, g);
   }
@@ -718,8 +727,8 @@ template <int kGroup>
 constexpr int cta_threads() {
   return kGroup <= 32 ? 256 : kGroup;
 }
-// On an SM.  More writing streams are slower (gradient of 65536 x 4000 bf16: 182 us,
-// with 1536 threads 227), and a teacher's row takes registers (its loss and gradient,
+// On an SM.  More writing streams are slower (gradient of 65536 x 4000 bf16: 178 us,
+// with 1536 threads some 25 % more), and a teacher's row takes registers (its loss and gradient,
 // 64 entries: 318 us, with 1024 threads 378).
 template <int kMode, bool kA, bool kB>
 constexpr int resident_threads() {
@@ -841,7 +850,7 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kMode,
       const T* x = row_at<T>(A, r);
       T* out = static_cast<T*>(A.grad) + r * n;
       if (!writes) zero_slice<T, kGroup>(out, n, g);
-      if (writes) write_slice<T, kGroup>(x, out, n, g, row.st.m, A.c, factor * inv_s);
+      if (writes) write_slice<T, kGroup, kA>(x, out, n, g, row.st.m, A.c, factor * inv_s);
       if (kA && next.counts) begun.st = slice_part<T, kGroup, kB>(row_at<T>(A, rn), n, g, A.c);
     } else if (next.counts) {
       begun.st = slice_part<T, kGroup, kB>(row_at<T>(A, rn), n, g, A.c);
