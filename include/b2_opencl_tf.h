@@ -394,8 +394,8 @@ int b2_adam_update(b2_stream_t stream, int num_tensors, float* const* params,
  * Weights are null (all 1), float32 (4) or one byte each (1: 0 or not 0).  What
  * belongs to a weight of 0 is not looked at.  A row of scores with a NaN or
  * +inf, or with -inf only, has no softmax: its results are NaN (unless it
- * does not count).  Results are deterministic.  Sums and softmax statistics
- * are held in 32 bits or more. */
+ * does not count).  Gradients must not overlap the scores.  Results are
+ * deterministic.  Sums and softmax statistics are held in 32 bits or more. */
 
 typedef enum b2_dtype { B2_FLOAT32 = 0, B2_FLOAT16 = 1, B2_BFLOAT16 = 2 } b2_dtype_t;
 

@@ -14,9 +14,12 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
+#include <cstring>
 #include <optional>
+#include <sstream>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "b2_opencl_tf.h"
 

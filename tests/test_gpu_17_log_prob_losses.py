@@ -808,3 +808,41 @@ def test_train_step_with_a_loss(otf, kind):
     for got, want in zip(model.parameters(), torch.autograd.grad(ref, params)):
         # the products' fp32 tolerance, 5e-6 of the largest value each way
         assert float((got.grad - want).norm() / want.norm()) <= 2e-5
+
+
+def test_errors_of_a_backward_pass(otf):
+    """What fails in the backward pass, on autograd's own thread, is raised where the gradient was asked for: scores
+    changed since the forward pass, and a wait of another op that ran out (a matrix product given 1 ns; it gives up)."""
+    from opencl_tf import errors, raw_ops
+    x = torch.randn(40, 5000, device="cuda", requires_grad=True)
+    t = torch.randint(0, 5000, (40,), device="cuda")
+    y = x * 1
+    lp = otf.losses.token_log_probs(y, t).sum()
+    y.detach().add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(lp, x)
+
+    lp = otf.losses.token_log_probs(x, t).sum()
+    want, = torch.autograd.grad(lp, x, retain_graph=True)
+    a, w, b = torch.randn(512, 4096, device="cuda"), torch.randn(4096, 96, device="cuda"), torch.zeros(96, device="cuda")
+    before = otf.device_timeouts()
+    try:
+        otf.set_wait_limit_ns(1)
+        for _ in range(5):
+            try:
+                raw_ops.opencl_dense(a, w, b)
+            except errors.DeadlineExceededError:
+                pass
+            torch.cuda.synchronize()
+            if otf.device_timeouts() > before:
+                break
+    finally:
+        otf.set_wait_limit_ns(0)
+    with pytest.raises(errors.DeadlineExceededError):
+        torch.autograd.grad(lp, x, retain_graph=True)
+    with pytest.raises(errors.DeadlineExceededError):
+        otf.losses.token_log_probs(x, t)
+    with pytest.raises(errors.DeadlineExceededError):
+        otf.stream_status()
+    again, = torch.autograd.grad(lp, x)
+    assert torch.equal(again, want)
