@@ -58,7 +58,8 @@ def _compile(src: Path, force: bool, ptxas_v: bool) -> tuple[Path, str]:
 
 
 def _compile_binding(src: Path, force: bool) -> Path:
-    """``opencl_tf/_<stem>.so`` from ``torch_binding/<stem>.cpp``."""
+    """``opencl_tf/_<stem>.so`` from ``torch_binding/<stem>.cpp``, by the system's compiler: another one (from
+    ``CXX``, say) may link parts of a libstdc++ beside the one that torch has loaded."""
     out = PKG / "opencl_tf" / f"_{src.stem}.so"
     newest = max(p.stat().st_mtime for p in (src, INCLUDE / "b2_opencl_tf.h"))
     if not force and out.exists() and out.stat().st_mtime >= newest:
@@ -68,7 +69,8 @@ def _compile_binding(src: Path, force: bool) -> Path:
     cuda = Path(nvcc()).resolve().parent.parent
     includes = [a for p in cpp_extension.include_paths() for a in ("-isystem", p)]
     libs = [a for p in cpp_extension.library_paths() for a in ("-L", p)]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+    system = "/usr/bin/g++"
+    cmd = [system if os.path.exists(system) else "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
            f"-DTORCH_EXTENSION_NAME=_{src.stem}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *includes, "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"],
            "-I", str(INCLUDE), str(src), "-o", str(out), *libs, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",

@@ -16,7 +16,6 @@
 
 #include <cstring>
 #include <optional>
-#include <sstream>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -106,11 +105,12 @@ std::string names_of(unsigned types) {
   return s;
 }
 
-template <class T>
-std::string text(const T& v) {
-  std::ostringstream s;
-  s << v;
-  return s.str();
+std::string text(at::ScalarType t) { return c10::toString(t); }
+
+std::string text(c10::IntArrayRef shape) {
+  std::string s = "[";
+  for (const int64_t n : shape) s += (s.size() > 1 ? ", " : "") + std::to_string(n);
+  return s + "]";
 }
 
 b2_dtype_t dtype_of(const Tensor& t) {

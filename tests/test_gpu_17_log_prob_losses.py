@@ -602,6 +602,65 @@ def test_no_token_counts(otf):
     assert all(not o.any() for o in got)
 
 
+REFUSED = {
+    "token_log_probs": [(dict(logits=lambda a: a.double()), "logits must be float32"),
+                        (dict(logits=lambda a: a[:, :0]), "at least one class"),
+                        (dict(logits=lambda a: a.sum()), "classes"),
+                        (dict(logits=lambda a: a.cpu()), "CUDA device"),
+                        (dict(targets=lambda a: a.float()), "targets must be int32, int64"),
+                        (dict(targets=lambda a: a[:3]), "targets must have shape"),
+                        (dict(targets=lambda a: a.cpu()), "CUDA device")],
+    "distillation_loss": [(dict(teacher_ids=lambda a: a[:3]), "teacher_ids must be"),
+                          (dict(teacher_ids=lambda a: a.float()), "teacher_ids must be int32, int64"),
+                          (dict(teacher_logits=lambda a: a[:, :2]), "teacher_logits must have shape"),
+                          (dict(teacher_logits=lambda a: a.double()), "teacher_logits must be float32"),
+                          (dict(teacher_ids=lambda a: a[:, :0], teacher_logits=lambda a: a[:, :0]), "entries"),
+                          (dict(teacher_ids=lambda a: a.repeat(1, 342), teacher_logits=lambda a: a.repeat(1, 342)),
+                           "entries"),
+                          (dict(weights=lambda a: torch.ones(3, device="cuda")), "weights must have shape"),
+                          (dict(weights=lambda a: torch.ones(4, device="cuda").long()), "weights must be float32, bool"),
+                          (dict(temperature=lambda a: 0.0), "temperature"),
+                          (dict(temperature=lambda a: math.nan), "temperature"),
+                          (dict(logits=lambda a: a[:0], teacher_ids=lambda a: a[:0], teacher_logits=lambda a: a[:0]),
+                           "no rows")],
+    "distillation_loss_with_grad": [(dict(grad_loss=lambda a: torch.ones(2, device="cuda")), "grad_loss must be"),
+                                    (dict(grad_loss=lambda a: 2.0), "grad_loss must be")],
+    "preference_loss": [(dict(log_probs=lambda a: a.half()), "log_probs must be float32"),
+                        (dict(offsets=lambda a: a[:4]), "offsets"), (dict(offsets=lambda a: a[:1]), "offsets"),
+                        (dict(offsets=lambda a: a[None]), "offsets"), (dict(offsets=lambda a: a.float()), "offsets"),
+                        (dict(ref_log_probs=lambda a: torch.ones(5, device="cuda")), "ref_log_probs must have shape"),
+                        (dict(mask=lambda a: torch.ones(4)), "CUDA device"),
+                        (dict(beta=lambda a: math.inf), "beta"),
+                        (dict(label_smoothing=lambda a: 0.6), "label_smoothing")],
+    "policy_loss": [(dict(old_log_probs=lambda a: a[:2]), "old_log_probs must have shape"),
+                    (dict(advantages=lambda a: a.half()), "advantages must be float32"),
+                    (dict(clip_low=lambda a: -0.1), "clip"), (dict(clip_high=lambda a: math.nan), "clip"),
+                    (dict(kl_coef=lambda a: math.inf), "kl_coef")],
+    "policy_loss_with_grad": [(dict(targets=lambda a: a[:, None]), "targets must have shape"),
+                              (dict(grad_loss=lambda a: torch.ones((), device="cuda").half()), "grad_loss must be")],
+}
+
+
+@pytest.mark.parametrize("name,change,words", [(n, *c) for n, l in REFUSED.items() for c in l])
+def test_refusals(otf, name, change, words):
+    """Wrong types, shapes and values are refused before anything runs."""
+    from opencl_tf import errors
+    x, t, lp = torch.zeros(4, 10, device="cuda"), torch.zeros(4, device="cuda").long(), torch.zeros(4, device="cuda")
+    calls = {
+        "token_log_probs": dict(logits=x, targets=t),
+        "distillation_loss": dict(logits=x, teacher_ids=t[:, None].repeat(1, 3), teacher_logits=x[:, :3]),
+        "preference_loss": dict(log_probs=lp, offsets=torch.arange(5, device="cuda")),
+        "policy_loss": dict(log_probs=lp, old_log_probs=lp, advantages=lp),
+        "policy_loss_with_grad": dict(logits=x, targets=t, old_log_probs=lp, advantages=lp),
+    }
+    args = dict(calls.get(name, calls["distillation_loss"]))
+    getattr(otf.losses, name)(**args)
+    for k, f in change.items():
+        args[k] = f(args.get(k))
+    with pytest.raises(errors.InvalidArgumentError, match=words):
+        getattr(otf.losses, name)(**args)
+
+
 # ---------------------------------------------------------------- together
 
 def test_gradients_against_differences(otf):
