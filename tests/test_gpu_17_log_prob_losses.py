@@ -905,3 +905,39 @@ def test_errors_of_a_backward_pass(otf):
         otf.stream_status()
     again, = torch.autograd.grad(lp, x)
     assert torch.equal(again, want)
+
+
+def test_calls_of_two_threads(otf):
+    """Losses and gradients of two threads, each on a stream of its own, and a backward pass on the calling thread."""
+    import threading
+    inputs = [scores(60, 7001 + 100 * i, "bf16", i, dead=False) for i in range(2)]
+    old, adv = torch.zeros(60, device="cuda") - 9, torch.randn(60, device="cuda")
+
+    def step(x, t):
+        leaf = x.clone().requires_grad_()
+        loss = otf.losses.policy_loss(otf.losses.token_log_probs(leaf, t), old, adv)[0]
+        return loss.detach(), *torch.autograd.grad(loss, leaf)
+
+    want = [step(*a) for a in inputs]
+    torch.cuda.synchronize()
+    got, failed = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    got[i].append(step(*inputs[i]))
+            torch.cuda.synchronize()
+        except BaseException as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed, failed
+    with torch.autograd.set_multithreading_enabled(False):
+        got[0].append(step(*inputs[0]))
+    for w, g in zip(want, got):
+        assert len(g) >= 30 and all(torch.equal(a, b) for one in g for a, b in zip(w, one))
