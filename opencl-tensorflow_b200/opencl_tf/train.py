@@ -28,6 +28,7 @@ import torch.distributed as dist
 from torch.distributed import distributed_c10d as c10d
 
 from . import _library as _L
+from . import errors
 from ._library import set_reserved_sms, step_ops
 from .optimizers import Adam
 
@@ -282,8 +283,26 @@ def _buffers_like(y):
     return tuple(torch.empty_like(t) for t in y) if isinstance(y, tuple) else torch.empty_like(y)
 
 
-def _copy_into(buffers, y, non_blocking: bool = False) -> None:
-    pairs = zip(buffers, y) if isinstance(buffers, tuple) else ((buffers, y),)
+def _copies(buffers, given, what: str) -> list:
+    """(buffer, tensor) pairs by which a step's input or targets go into the buffers of a captured graph.  What has
+    another form than the buffers is refused: a shorter tuple would leave the last batch's values in the rest of them,
+    and a copy broadcasts.  The types of a tuple's tensors are the captured ones; a single tensor may be of another type
+    that torch converts (float64 images, say), but not to one that drops fractions."""
+    several = isinstance(buffers, tuple)
+    bs, ts = (buffers, given) if several else ((buffers,), (given,))
+    fits = isinstance(ts, tuple) and len(bs) == len(ts) and all(
+        isinstance(t, torch.Tensor) and t.shape == b.shape
+        and (t.dtype == b.dtype or (not several and torch.can_cast(t.dtype, b.dtype))) for b, t in zip(bs, ts))
+    if not fits:
+        def form(v):
+            if isinstance(v, (tuple, list)):
+                return f"{type(v).__name__}({', '.join(form(t) for t in v)})"
+            return f"{v.dtype}{list(v.shape)}" if isinstance(v, torch.Tensor) else type(v).__name__
+        raise errors.InvalidArgumentError(f"the step was captured with {what} {form(buffers)}, got {form(given)}")
+    return list(zip(bs, ts))
+
+
+def _copy(pairs, non_blocking: bool = False) -> None:
     for b, t in pairs:
         if t.data_ptr() != b.data_ptr():
             b.copy_(t, non_blocking=non_blocking)
@@ -296,7 +315,8 @@ class TrainStep:
     model's output and the targets that returns a device scalar, or a tuple
     that begins with one, made of differentiable ops that a CUDA graph can
     hold (the ones of ``losses``, for instance).  ``y`` is what it needs: a tensor
-    or a tuple of tensors, e.g. a teacher's (classes, logits).
+    or a tuple of tensors, e.g. a teacher's (classes, logits).  A captured step
+    takes inputs and targets of the form that it was captured with, and refuses others.
 
     ``reserved_sms``: with more than one rank, SMs kept free of the library's
     persistent tensor-core kernels so that NCCL's all-reduce kernels (and the
@@ -375,7 +395,7 @@ class TrainStep:
         self.static_x = torch.empty_like(x)
         self.static_y = _buffers_like(y)
         self.static_x.copy_(x)
-        _copy_into(self.static_y, y)
+        _copy(_copies(self.static_y, y, "targets"))
         side = torch.cuda.Stream(device=x.device)
         side.wait_stream(torch.cuda.current_stream(x.device))
         with torch.cuda.stream(side):
@@ -394,9 +414,7 @@ class TrainStep:
         if self.graph is None:
             self._capture(x, y)
         else:
-            if x.data_ptr() != self.static_x.data_ptr():
-                self.static_x.copy_(x, non_blocking=True)
-            _copy_into(self.static_y, y, non_blocking=True)
+            _copy(_copies(self.static_x, x, "input") + _copies(self.static_y, y, "targets"), non_blocking=True)
         self.graph.replay()
         return self.static_loss
 
@@ -414,7 +432,7 @@ class TrainStep:
             self.static_x1 = torch.empty_like(self.static_x)
             self.static_y1 = _buffers_like(self.static_y)
             self.static_x1.copy_(self.static_x)
-            _copy_into(self.static_y1, self.static_y)
+            _copy(_copies(self.static_y1, self.static_y, "targets"))
             torch.cuda.current_stream(self.static_x.device).synchronize()
             self.graph1 = torch.cuda.CUDAGraph()
             self.zero_grad()

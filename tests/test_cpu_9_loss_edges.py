@@ -1,0 +1,30 @@
+"""What the training step and the losses over rows of class scores refuse or survive, without a GPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from opencl_tf import errors
+
+
+def test_targets_of_another_form_than_the_captured():
+    """A captured step's buffers take what has their form; anything else is refused and leaves them as they were."""
+    from opencl_tf import train
+    ids, y = torch.arange(12).view(4, 3), torch.randn(4, 3)
+    buffers = (torch.zeros_like(ids), torch.zeros_like(y))
+    train._copy(train._copies(buffers, (ids, y), "targets"))
+    assert torch.equal(buffers[0], ids) and torch.equal(buffers[1], y)
+    for bad in ((ids + 1,), ids + 1, y + 1, (y, ids), (ids + 1, y[:1]), (ids[:2], y[:2]), (ids + 1, y, y), (ids + 1, y.half()),
+                (ids.int(), y), [ids + 1, y], (ids + 1, None), None, ()):
+        with pytest.raises(errors.InvalidArgumentError, match="captured with targets"):
+            train._copy(train._copies(buffers, bad, "targets"))
+        assert torch.equal(buffers[0], ids) and torch.equal(buffers[1], y)
+    one = torch.zeros(4, 3)
+    for good in (y, y.double(), torch.ones(4, 3, dtype=torch.uint8), y.t().contiguous().t()):  # converted, as ever
+        train._copy(train._copies(one, good, "input"))
+        assert torch.equal(one, good.float())
+    for bad in (y[:1], y[0], y[None], y[:, :1], torch.tensor(1.0), (y,), [y], None):
+        with pytest.raises(errors.InvalidArgumentError, match="captured with input"):
+            train._copy(train._copies(one, bad, "input"))
+    with pytest.raises(errors.InvalidArgumentError):
+        train._copy(train._copies(buffers[0], y, "input"))  # would drop fractions
