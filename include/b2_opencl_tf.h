@@ -395,7 +395,8 @@ int b2_adam_update(b2_stream_t stream, int num_tensors, float* const* params,
  * belongs to a weight of 0 is not looked at.  A row of scores with a NaN or
  * +inf, or with -inf only, has no softmax: its results are NaN (unless it
  * does not count).  Gradients must not overlap the scores.  Results are
- * deterministic.  Sums and softmax statistics are held in 32 bits or more. */
+ * deterministic.  Sums and softmax statistics are held in 32 bits or more.
+ * Pointers are aligned to their elements; row_stats to 8 bytes, which is checked. */
 
 typedef enum b2_dtype { B2_FLOAT32 = 0, B2_FLOAT16 = 1, B2_BFLOAT16 = 2 } b2_dtype_t;
 
@@ -407,8 +408,8 @@ typedef struct b2_logits {
 } b2_logits_t;
 
 /* log_probs[r] = x[r, t] - log sum_j exp(x[r, j]), t = targets[r]; 0 for an
- * ignored target.  row_stats: [rows][2] floats for the gradient (the row's
- * maximum m and sum_j exp(x_j - m)), or null. */
+ * ignored target.  row_stats: [rows][2] floats, 8-byte aligned, for the gradient
+ * (the row's maximum m and sum_j exp(x_j - m)), or null. */
 int b2_token_log_probs(b2_stream_t stream, const b2_logits_t* logits,
                        const void* targets, int target_bytes, float* log_probs,
                        float* row_stats);

@@ -350,6 +350,12 @@ int weight_ok(const void* w, int bytes, const char* what) {
   return B2_OK;
 }
 
+// Statistics are read and written as pairs of floats, and the sum behind them in 64 bits.
+int stats_ok(const float* row_stats, const char* what) {
+  B2_REQUIRE((reinterpret_cast<uintptr_t>(row_stats) & 7) == 0, "%s: row_stats must be 8-byte aligned", what);
+  return B2_OK;
+}
+
 int sum_weights(cudaStream_t s, const void* w, int bytes, int64_t rows, double* total, const char* what) {
   weight_sum_kernel<<<kSumCtas, kSumThreads, 0, s>>>(w, bytes, rows, total);
   return check_launch(s, what);
@@ -368,6 +374,7 @@ int b2_token_log_probs(b2_stream_t stream, const b2_logits_t* logits, const void
   RowArgs a;
   B2_RETURN_IF_ERROR(row_args(logits, "token_log_probs", &a));
   B2_RETURN_IF_ERROR(index_ok(target_bytes, "token_log_probs", "targets"));
+  B2_RETURN_IF_ERROR(stats_ok(row_stats, "token_log_probs"));
   if (a.rows == 0) return B2_OK;
   B2_REQUIRE(targets != nullptr && log_probs != nullptr, "token_log_probs: null pointer");
   const DeviceInfo* d = nullptr;
@@ -385,6 +392,7 @@ int b2_token_log_probs_grad(b2_stream_t stream, const b2_logits_t* logits, const
   RowArgs a;
   B2_RETURN_IF_ERROR(row_args(logits, "token_log_probs_grad", &a));
   B2_RETURN_IF_ERROR(index_ok(target_bytes, "token_log_probs_grad", "targets"));
+  B2_RETURN_IF_ERROR(stats_ok(row_stats, "token_log_probs_grad"));
   if (a.rows == 0) return B2_OK;
   B2_REQUIRE(targets != nullptr && row_stats != nullptr && grad_log_probs != nullptr && grad_logits != nullptr,
              "token_log_probs_grad: null pointer");
@@ -434,7 +442,7 @@ int b2_distillation_loss(b2_stream_t stream, const b2_logits_t* logits, const vo
   B2_RETURN_IF_ERROR(distill_args(logits, teacher_ids, id_bytes, teacher_logits, teacher_dtype, top, weights,
                                   weight_bytes, temperature, "distillation_loss", &a));
   B2_REQUIRE(loss != nullptr, "distillation_loss: null pointer");
-  B2_REQUIRE((reinterpret_cast<uintptr_t>(row_stats) & 7) == 0, "distillation_loss: row_stats must be 8-byte aligned");
+  B2_RETURN_IF_ERROR(stats_ok(row_stats, "distillation_loss"));
   const DeviceInfo* d = nullptr;
   B2_RETURN_IF_ERROR(device_info(&d));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -469,6 +477,7 @@ int b2_distillation_loss_grad(b2_stream_t stream, const b2_logits_t* logits, con
                                   weight_bytes, temperature, "distillation_loss_grad", &a));
   B2_REQUIRE(row_stats != nullptr && grad_loss != nullptr && grad_logits != nullptr,
              "distillation_loss_grad: null pointer");
+  B2_RETURN_IF_ERROR(stats_ok(row_stats, "distillation_loss_grad"));
   const DeviceInfo* d = nullptr;
   B2_RETURN_IF_ERROR(device_info(&d));
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -28,3 +28,17 @@ def test_targets_of_another_form_than_the_captured():
             train._copy(train._copies(one, bad, "input"))
     with pytest.raises(errors.InvalidArgumentError):
         train._copy(train._copies(buffers[0], y, "input"))  # would drop fractions
+
+
+def test_misaligned_row_stats_are_refused():
+    """Statistics are stored as pairs of floats: an address that is no multiple of 8 is refused before any launch."""
+    import ctypes
+
+    from opencl_tf import _library as L
+    lib, x = L._lib, ctypes.byref(L.Logits(data=64, dtype=0, outer=1, inner=4, classes=10, outer_stride=0, inner_stride=10))
+    P, odd = ctypes.c_void_p(64), ctypes.c_void_p(68)  # never looked at
+    for name, args in (("token_log_probs", (P, 8, P, odd)), ("token_log_probs_grad", (P, 8, odd, P, P)),
+                       ("distillation_loss", (P, 8, P, 0, 4, None, 0, 1.0, P, odd, None, None)),
+                       ("distillation_loss_grad", (P, 8, P, 0, 4, None, 0, 1.0, odd, P, P))):
+        assert getattr(lib, "b2_" + name)(None, x, *args) == 1
+        assert L._lib.b2_last_error().decode() == name + ": row_stats must be 8-byte aligned"
