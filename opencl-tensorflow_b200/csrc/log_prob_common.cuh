@@ -73,8 +73,8 @@ __device__ __forceinline__ float weight_at(const void* w, int bytes, int64_t i) 
 }
 
 struct PolicyTerm {
-  double value;
-  float slope, kl;
+  double value, kl;
+  float slope;
   bool cut;
 };
 
@@ -83,8 +83,9 @@ struct PolicyTerm {
 // within 1e-5 of a border, where its rounding could put it on the other side, is
 // looked at again in 64.  The value is put together in 64 bits: advantages of both
 // signs cancel in the mean, and a border or coefficient rounded to 32 bits would
-// move all cut tokens' terms the same way.  exp(d) - d - 1 is its series for
-// |d| <= 1, where the subtraction would cancel.
+// move all cut tokens' terms the same way.  The KL term exp(d) - d - 1 and its slope
+// are in 64 bits too, which hold exp(d) past d = 88.7; where its coefficient is 0 it
+// is only reported, and a term that is infinite all the same touches nothing else.
 template <bool kWide>
 __device__ __forceinline__ PolicyTerm policy_term(float lp, const PolicyToken& t, const PolicyClip& c) {
   PolicyTerm p;
@@ -100,26 +101,34 @@ __device__ __forceinline__ PolicyTerm policy_term(float lp, const PolicyToken& t
   // Where it is not cut, the unclipped term is the larger one.
   p.value = -(p.cut ? (above ? c.high : c.low) : ratio) * (double)adv;
   p.slope = p.cut ? 0.0f : (float)-ratio * adv;
-  p.kl = 0.0f;
+  p.kl = 0.0;
   if (t.has_ref) {
-    const float d = t.ref_lp - lp;
-    if (fabsf(d) <= 1.0f) {
-      float s = 1.0f / 39916800.0f;  // sum of d^(k - 2) / k!, k = 2 .. 11
-      s = fmaf(s, d, 1.0f / 3628800.0f);
-      s = fmaf(s, d, 1.0f / 362880.0f);
-      s = fmaf(s, d, 1.0f / 40320.0f);
-      s = fmaf(s, d, 1.0f / 5040.0f);
-      s = fmaf(s, d, 1.0f / 720.0f);
-      s = fmaf(s, d, 1.0f / 120.0f);
-      s = fmaf(s, d, 1.0f / 24.0f);
-      s = fmaf(s, d, 1.0f / 6.0f);
-      s = fmaf(s, d, 0.5f);
+    const double d = (double)t.ref_lp - (double)lp;
+    double rise;  // exp(d) - 1
+    if (fabs(d) <= 1.0) {
+      // exp(d) - d - 1 as its series, where the subtraction would cancel: the sum of
+      // d^(k - 2) / k!, k = 2 .. 11, leaves out less than 1e-8 of it
+      double s = 1.0 / 39916800.0;
+      s = fma(s, d, 1.0 / 3628800.0);
+      s = fma(s, d, 1.0 / 362880.0);
+      s = fma(s, d, 1.0 / 40320.0);
+      s = fma(s, d, 1.0 / 5040.0);
+      s = fma(s, d, 1.0 / 720.0);
+      s = fma(s, d, 1.0 / 120.0);
+      s = fma(s, d, 1.0 / 24.0);
+      s = fma(s, d, 1.0 / 6.0);
+      s = fma(s, d, 0.5);
       p.kl = s * d * d;
+      rise = d + p.kl;
     } else {
-      p.kl = expf(d) - d - 1.0f;
+      const double e = exp(d);
+      p.kl = isinf(e) ? e : e - d - 1.0;  // d itself may be infinite
+      rise = e - 1.0;
     }
-    p.value += c.kl_coef * (double)p.kl;
-    p.slope = fmaf(-(float)c.kl_coef, d + p.kl, p.slope);
+    if (c.kl_coef != 0.0) {
+      p.value += c.kl_coef * p.kl;
+      p.slope = (float)((double)p.slope - c.kl_coef * rise);
+    }
   }
   return p;
 }

@@ -95,3 +95,78 @@ def test_targets_of_another_form_than_the_captured(otf):
     b, a = run(False), run(True)
     for x, y in zip((*a[0], *a[1]), (*b[0], *b[1])):
         assert torch.equal(x, y)
+
+
+def _policy_forms(otf, x, t, old, adv, ref, **kw):
+    """(loss, mean KL, share, gradient of the log-probabilities) of the loss from log-probabilities, then (loss, mean KL,
+    share, gradient of the scores) of the one from the scores."""
+    leaf = otf.losses.token_log_probs(x, t).requires_grad_()
+    out = otf.losses.policy_loss(leaf, old, adv, ref_log_probs=ref, **kw)
+    grad, = torch.autograd.grad(out[0], leaf)
+    return leaf.detach(), (*[o.detach() for o in out], grad), otf.losses.policy_loss_with_grad(x, t, old, adv,
+                                                                                               ref_log_probs=ref, **kw)
+
+
+@pytest.mark.parametrize("classes", [16, 32768])
+def test_kl_of_tokens_far_from_the_reference(otf, classes):
+    """exp(d) past fp32's range: where kl_coef is 0, loss and gradient are those of no KL term, and the mean KL, which
+    fp32 holds, is right; where it is not, the term is its 64-bit value."""
+    n = 128
+    x, t = uniform_scores(n, classes)
+    lp = otf.losses.token_log_probs(x, t)
+    old, adv = lp + 0.1, torch.linspace(-1, 1, n, device="cuda")
+    ref = lp.clone()
+    ref[5] += 90.0  # exp(90) is 1.2e39, the mean of 128 such terms and zeros 9.5e36
+    for kl_coef in (0.0, 1e-30):
+        lp, parts, fused = _policy_forms(otf, x, t, old, adv, ref, kl_coef=kl_coef)
+        want = policy_definition(lp, old, adv, ref, kl_coef=kl_coef)
+        # terms in 64 bits (their series to 1e-8), the store's half step; the gradient: slope, 1 / sum and product.
+        # The advantages add up to 0, so without a KL term the loss is 0 but for its terms' roundings, each 8 * 2^-53
+        # of less than 1 in both sides
+        for got in (parts, fused):
+            for g, w in zip(got[:3], want):
+                near(g, w, 2 * U, 8 * 2.0 ** -53)
+        near(parts[3], want[3], 4 * U)
+        assert bool(fused[3].isfinite().all())
+        # of the scores: factor * (p - q) with p = 1 / classes exact but for its quotient
+        p = torch.full((n, classes), 1.0 / classes, device="cuda", dtype=torch.float64)
+        p.scatter_add_(1, t[:, None], torch.full((n, 1), -1.0, device="cuda", dtype=torch.float64))
+        near(fused[3], -want[3][:, None] * p, 8 * U)
+
+
+@pytest.mark.parametrize("classes", [40, 20001])
+def test_kl_of_an_excluded_token(otf, classes):
+    """A token that the scores exclude (log-probability -inf) has an infinite KL, which is only reported where kl_coef
+    is 0; one that the reference excludes has a finite slope."""
+    x = torch.randn(6, classes, device="cuda")
+    t = torch.arange(6, device="cuda")
+    x[1, 1] = -math.inf
+    old, adv, ref = torch.full((6,), -3.0, device="cuda"), torch.ones(6, device="cuda"), torch.full((6,), -3.0, device="cuda")
+    lp, with_ref, fused = _policy_forms(otf, x, t, old, adv, ref)
+    _, without, fused_without = _policy_forms(otf, x, t, old, adv, None)
+    assert float(lp[1]) == -math.inf and float(with_ref[1]) == math.inf and float(fused[1]) == math.inf
+    for a, b in ((with_ref, without), (fused, fused_without)):
+        for i in (0, 2, 3):
+            assert torch.equal(a[i], b[i]) and bool(a[i].isfinite().all())
+    x = torch.randn(6, classes, device="cuda")
+    ref[2] = -math.inf
+    lp, parts, fused = _policy_forms(otf, x, t, old, adv, ref, kl_coef=0.5)
+    assert float(parts[0]) == math.inf and float(fused[0]) == math.inf
+    near(parts[3], policy_definition(lp, old, adv, ref, kl_coef=0.5)[3], 4 * U)
+    assert bool(fused[3].isfinite().all())
+
+
+def test_kl_slopes_are_exact_to_their_store(otf):
+    """Slopes kl_coef (1 - exp(d)) for d from 1e-6 to 20 either way: the slope's, 1 / sum's and the product's half
+    step, and the last one; the mean of the terms: its store alone."""
+    d = torch.logspace(-6, math.log10(20.0), 4001, dtype=torch.float64)
+    d = torch.cat([d, -d]).cuda()
+    lp = -torch.rand(d.numel(), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 5
+    ref, zero = (lp.double() + d).float(), torch.zeros_like(lp)
+    leaf = lp.clone().requires_grad_()
+    loss, kl, _ = otf.losses.policy_loss(leaf, lp, zero, ref_log_probs=ref, kl_coef=0.25)
+    grad, = torch.autograd.grad(loss, leaf)
+    want = policy_definition(lp, lp, zero, ref, kl_coef=0.25)
+    near(kl, want[1], U + 2e-8)
+    near(loss, want[0], U + 2e-8)
+    near(grad, want[3], 4 * U + 2e-8)
