@@ -79,24 +79,18 @@ struct PolicyTerm {
 };
 
 // One token's term of the clipped policy loss and its slope in the token's
-// log-probability.  kWide: the ratio is taken in 64 bits; else in 32, and only one
-// within 1e-5 of a border, where its rounding could put it on the other side, is
-// looked at again in 64.  The value is put together in 64 bits: advantages of both
-// signs cancel in the mean, and a border or coefficient rounded to 32 bits would
-// move all cut tokens' terms the same way.  The KL term exp(d) - d - 1 and its slope
+// log-probability.  Ratio and value are in 64 bits: advantages of both signs cancel
+// in the mean, and a border or coefficient rounded to 32 bits would move all cut
+// tokens' terms the same way.  The log-probability is the fp32 number that
+// b2_token_log_probs gives, in the loss from the scores too: where the old one is that
+// number, the ratio is exactly 1.  The KL term exp(d) - d - 1 and its slope
 // are in 64 bits too, which hold exp(d) past d = 88.7; where its coefficient is 0 it
 // is only reported, and a term that is infinite all the same touches nothing else.
-template <bool kWide>
 __device__ __forceinline__ PolicyTerm policy_term(float lp, const PolicyToken& t, const PolicyClip& c) {
   PolicyTerm p;
   const float adv = t.advantage;
-  const double ratio = kWide ? exp((double)lp - (double)t.old_lp) : (double)expf(lp - t.old_lp);
-  bool above = ratio > c.high, below = ratio < c.low;
-  if (!kWide && (fabs(ratio - c.high) <= 1e-5 * c.high || fabs(ratio - c.low) <= 1e-5)) {
-    const double exact = exp((double)lp - (double)t.old_lp);
-    above = exact > c.high;
-    below = exact < c.low;
-  }
+  const double ratio = exp((double)lp - (double)t.old_lp);
+  const bool above = ratio > c.high, below = ratio < c.low;
   p.cut = (adv > 0.0f && above) || (adv < 0.0f && below);
   // Where it is not cut, the unclipped term is the larger one.
   p.value = -(p.cut ? (above ? c.high : c.low) : ratio) * (double)adv;

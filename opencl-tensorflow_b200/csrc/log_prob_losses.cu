@@ -237,7 +237,7 @@ __device__ __forceinline__ void policy_part(const PolicyArgs& A, int64_t first, 
     float slope = 0.0f;
     if (w != 0.0f) {
       const PolicyTerm t =
-          policy_term<true>(A.lp[n], PolicyToken{A.old_lp[n], A.advantages[n], has_ref ? A.ref_lp[n] : 0.0f, has_ref},
+          policy_term(A.lp[n], PolicyToken{A.old_lp[n], A.advantages[n], has_ref ? A.ref_lp[n] : 0.0f, has_ref},
                             A.clip);
       slope = w * t.slope;
       v[0] += (double)w * t.value;

@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kS
   // ---- the row's end
   if (kMode == kPolicy) {
     if (helper) {
-      const PolicyTerm t = policy_term<false>(target >= 0 ? log_prob(x_target, st) : 0.0f, token, A.clip);
+      const PolicyTerm t = policy_term(target >= 0 ? log_prob(x_target, st) : 0.0f, token, A.clip);
       if (lane == 0) {
         factor_s = -share * t.slope;
         if (rank == 0) store_policy(A, r, t, w);
@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kMode,
       } else {
         if (g == 0) {
           const float lp = row.real ? log_prob(row.x_target, row.st) : 0.0f;
-          const PolicyTerm t = policy_term<false>(lp, policy_token(A, r), A.clip);
+          const PolicyTerm t = policy_term(lp, policy_token(A, r), A.clip);
           store_policy(A, r, t, now.w);
           factor = -now.w * unit * t.slope;
           if (kCta) factor_s[buf] = factor;

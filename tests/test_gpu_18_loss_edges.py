@@ -27,7 +27,7 @@ def policy_definition(lp, old, adv, ref=None, low=0.2, high=0.2, kl_coef=0.0):
     n = lp.numel()
     r = torch.exp(lp - old)
     cut = ((adv > 0) & (r > 1 + high)) | ((adv < 0) & (r < 1 - low))
-    value = -torch.where(cut, torch.where(adv > 0, 1 + high, 1 - low), r) * adv
+    value = -torch.where(cut, r.clamp(1 - low, 1 + high), r) * adv
     slope = torch.where(cut, torch.zeros_like(r), -r * adv)
     kl = torch.zeros_like(r)
     if ref is not None:
@@ -170,3 +170,24 @@ def test_kl_slopes_are_exact_to_their_store(otf):
     near(kl, want[1], U + 2e-8)
     near(loss, want[0], U + 2e-8)
     near(grad, want[3], 4 * U + 2e-8)
+
+
+@pytest.mark.parametrize("rows,classes", [(40001, 32), (300, 16384), (70, 131072)])
+def test_policy_loss_with_grad_of_cancelling_terms(otf, rows, classes):
+    """The mean of terms of both signs, clipped ones among them, that nearly cancel: from the scores it is as exact as
+    from log-probabilities."""
+    x, t = uniform_scores(rows, classes)
+    lp = otf.losses.token_log_probs(x, t)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    old = lp + 0.3 * torch.randn(rows, generator=g, device="cuda")
+    adv = torch.randn(rows, generator=g, device="cuda")
+    old[-1], adv[-1] = lp[-1], 0.0
+    total = policy_definition(lp, old, adv, high=0.28)[0] * rows
+    adv[-1] = total  # its ratio is 1
+    want = policy_definition(lp, old, adv, high=0.28)
+    assert abs(float(want[0])) < 1e-5 and float(want[2]) > 0.1
+    loss, _, share, grad = otf.losses.policy_loss_with_grad(x, t, old, adv, clip_low=0.2, clip_high=0.28)
+    # the result's half step, and per term the few 2^-53 of its exponential
+    near(loss, want[0], U, 8 * 2.0 ** -53 * float(adv.abs().sum()) / rows * 1.28)
+    near(share, want[2], U)
+    assert torch.equal(loss, otf.losses.policy_loss(lp, old, adv, clip_low=0.2, clip_high=0.28)[0])
