@@ -73,28 +73,28 @@ __device__ __forceinline__ float weight_at(const void* w, int bytes, int64_t i) 
 }
 
 struct PolicyTerm {
-  double value, kl;
-  float slope;
+  double value, slope, kl;
   bool cut;
 };
 
 // One token's term of the clipped policy loss and its slope in the token's
 // log-probability.  Ratio and value are in 64 bits: advantages of both signs cancel
 // in the mean, and a border or coefficient rounded to 32 bits would move all cut
-// tokens' terms the same way.  The log-probability is the fp32 number that
+// tokens' terms the same way.  So is the slope until its store: a ratio past 32 bits'
+// range times an advantage of 0 is 0.  The log-probability is the fp32 number that
 // b2_token_log_probs gives, in the loss from the scores too: where the old one is that
 // number, the ratio is exactly 1.  The KL term exp(d) - d - 1 and its slope
 // are in 64 bits too, which hold exp(d) past d = 88.7; where its coefficient is 0 it
 // is only reported, and a term that is infinite all the same touches nothing else.
 __device__ __forceinline__ PolicyTerm policy_term(float lp, const PolicyToken& t, const PolicyClip& c) {
   PolicyTerm p;
-  const float adv = t.advantage;
+  const double adv = (double)t.advantage;
   const double ratio = exp((double)lp - (double)t.old_lp);
   const bool above = ratio > c.high, below = ratio < c.low;
-  p.cut = (adv > 0.0f && above) || (adv < 0.0f && below);
+  p.cut = (adv > 0.0 && above) || (adv < 0.0 && below);
   // Where it is not cut, the unclipped term is the larger one.
-  p.value = -(p.cut ? (above ? c.high : c.low) : ratio) * (double)adv;
-  p.slope = p.cut ? 0.0f : (float)-ratio * adv;
+  p.value = -(p.cut ? (above ? c.high : c.low) : ratio) * adv;
+  p.slope = p.cut ? 0.0 : -ratio * adv;
   p.kl = 0.0;
   if (t.has_ref) {
     const double d = (double)t.ref_lp - (double)lp;
@@ -121,7 +121,7 @@ __device__ __forceinline__ PolicyTerm policy_term(float lp, const PolicyToken& t
     }
     if (c.kl_coef != 0.0) {
       p.value += c.kl_coef * p.kl;
-      p.slope = (float)((double)p.slope - c.kl_coef * rise);
+      p.slope -= c.kl_coef * rise;
     }
   }
   return p;

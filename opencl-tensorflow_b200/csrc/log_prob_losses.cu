@@ -239,7 +239,7 @@ __device__ __forceinline__ void policy_part(const PolicyArgs& A, int64_t first, 
       const PolicyTerm t =
           policy_term(A.lp[n], PolicyToken{A.old_lp[n], A.advantages[n], has_ref ? A.ref_lp[n] : 0.0f, has_ref},
                             A.clip);
-      slope = w * t.slope;
+      slope = (float)((double)w * t.slope);
       v[0] += (double)w * t.value;
       v[1] += (double)w * t.kl;
       v[2] += t.cut ? (double)w : 0.0;
@@ -302,10 +302,10 @@ __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)
 __global__ void __launch_bounds__(kTokenThreads)
     policy_grad_kernel(const float* __restrict__ grad_loss, const float* __restrict__ inv_total,
                        const float* __restrict__ slopes, int64_t tokens, float* __restrict__ grad) {
-  const float f = *grad_loss * *inv_total;
+  const double f = (double)*grad_loss * (double)*inv_total;
   for (int64_t n = (int64_t)blockIdx.x * kTokenThreads + threadIdx.x; n < tokens;
        n += (int64_t)gridDim.x * kTokenThreads)
-    grad[n] = slopes[n] == 0.0f ? 0.0f : f * slopes[n];
+    grad[n] = slopes[n] == 0.0f ? 0.0f : (float)(f * (double)slopes[n]);
 }
 
 // ----------------------------------------------------------------- entries

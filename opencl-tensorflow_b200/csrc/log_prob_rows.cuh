@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, kWarps > 8 ? 3 : kPass == kS
     if (helper) {
       const PolicyTerm t = policy_term(target >= 0 ? log_prob(x_target, st) : 0.0f, token, A.clip);
       if (lane == 0) {
-        factor_s = -share * t.slope;
+        factor_s = (float)(-(double)share * t.slope);
         if (rank == 0) store_policy(A, r, t, w);
       }
     }
@@ -827,7 +827,7 @@ __global__ void __launch_bounds__(cta_threads<kGroup>(), resident_threads<kMode,
           const float lp = row.real ? log_prob(row.x_target, row.st) : 0.0f;
           const PolicyTerm t = policy_term(lp, policy_token(A, r), A.clip);
           store_policy(A, r, t, now.w);
-          factor = -now.w * unit * t.slope;
+          factor = (float)(-(double)(now.w * unit) * t.slope);
           if (kCta) factor_s[buf] = factor;
         }
         if (!kCta) factor = __shfl_sync(lanes_mask<kLanes>(), factor, 0, kLanes);

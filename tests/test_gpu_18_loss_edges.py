@@ -191,3 +191,18 @@ def test_policy_loss_with_grad_of_cancelling_terms(otf, rows, classes):
     near(loss, want[0], U, 8 * 2.0 ** -53 * float(adv.abs().sum()) / rows * 1.28)
     near(share, want[2], U)
     assert torch.equal(loss, otf.losses.policy_loss(lp, old, adv, clip_low=0.2, clip_high=0.28)[0])
+
+
+@pytest.mark.parametrize("classes", [16, 32768])
+def test_an_advantage_of_zero_has_no_gradient(otf, classes):
+    """Whatever finite ratio the token has: exp(100) is past fp32's range, and 0 times it is 0."""
+    x, t = uniform_scores(64, classes)
+    old, adv = otf.losses.token_log_probs(x, t), torch.ones(64, device="cuda")
+    adv[::4] = 0.0
+    old[4] -= 100.0  # among those with advantage 0
+    lp, parts, fused = _policy_forms(otf, x, t, old, adv, None)
+    want = policy_definition(lp, old, adv)
+    for got in (parts, fused):
+        near(got[0], want[0], 2 * U)
+    near(parts[3], want[3], 4 * U)
+    assert not parts[3][::4].any() and not fused[3][::4].any() and bool(fused[3].isfinite().all())
