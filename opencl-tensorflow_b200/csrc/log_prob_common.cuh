@@ -72,59 +72,59 @@ __device__ __forceinline__ float weight_at(const void* w, int bytes, int64_t i) 
   return bytes == 4 ? static_cast<const float*>(w)[i] : (static_cast<const uint8_t*>(w)[i] != 0 ? 1.0f : 0.0f);
 }
 
+// One token of the clipped policy loss with a KL term, in 64 bits: advantages of both
+// signs cancel in the mean, and a border or coefficient rounded to 32 bits would move
+// all cut tokens' terms the same way; the ratio may pass 32 bits' range, and times an
+// advantage of 0 is 0 all the same.  The log-probability lp is the fp32 number that
+// b2_token_log_probs gives, in the loss from the scores too: where the old one is that
+// number, the ratio is exactly 1.
+struct PolicyKl {
+  double kl, rise;  // exp(d) - d - 1 and exp(d) - 1
+};
+__device__ __forceinline__ PolicyKl policy_kl(float lp, const PolicyToken& t) {
+  if (!t.has_ref) return PolicyKl{0.0, 0.0};
+  const double d = (double)t.ref_lp - (double)lp;
+  if (fabs(d) <= 1.0) {
+    // kl's series, where the subtraction would cancel: the sum of d^(k - 2) / k!,
+    // k = 2 .. 11, leaves out less than 1e-8 of it
+    double s = 1.0 / 39916800.0;
+    s = fma(s, d, 1.0 / 3628800.0);
+    s = fma(s, d, 1.0 / 362880.0);
+    s = fma(s, d, 1.0 / 40320.0);
+    s = fma(s, d, 1.0 / 5040.0);
+    s = fma(s, d, 1.0 / 720.0);
+    s = fma(s, d, 1.0 / 120.0);
+    s = fma(s, d, 1.0 / 24.0);
+    s = fma(s, d, 1.0 / 6.0);
+    s = fma(s, d, 0.5);
+    const double kl = s * d * d;
+    return PolicyKl{kl, d + kl};
+  }
+  const double e = exp(d);
+  return PolicyKl{isinf(e) ? e : e - d - 1.0, e - 1.0};  // d itself may be infinite
+}
+
 struct PolicyTerm {
-  double value, slope, kl;
+  double slope;  // in the token's log-probability
+  double held;   // the ratio, or the border that it is held at
   bool cut;
 };
-
-// One token's term of the clipped policy loss and its slope in the token's
-// log-probability.  Ratio and value are in 64 bits: advantages of both signs cancel
-// in the mean, and a border or coefficient rounded to 32 bits would move all cut
-// tokens' terms the same way.  So is the slope until its store: a ratio past 32 bits'
-// range times an advantage of 0 is 0.  The log-probability is the fp32 number that
-// b2_token_log_probs gives, in the loss from the scores too: where the old one is that
-// number, the ratio is exactly 1.  The KL term exp(d) - d - 1 and its slope
-// are in 64 bits too, which hold exp(d) past d = 88.7; where its coefficient is 0 it
-// is only reported, and a term that is infinite all the same touches nothing else.
-__device__ __forceinline__ PolicyTerm policy_term(float lp, const PolicyToken& t, const PolicyClip& c) {
-  PolicyTerm p;
-  const double adv = (double)t.advantage;
-  const double ratio = exp((double)lp - (double)t.old_lp);
+// Where the KL term's coefficient is 0 it is only reported: an infinite one touches
+// neither slope nor value.
+__device__ __forceinline__ PolicyTerm policy_term(const PolicyToken& t, const PolicyClip& c, double ratio, double rise) {
   const bool above = ratio > c.high, below = ratio < c.low;
-  p.cut = (adv > 0.0 && above) || (adv < 0.0 && below);
-  // Where it is not cut, the unclipped term is the larger one.
-  p.value = -(p.cut ? (above ? c.high : c.low) : ratio) * adv;
-  p.slope = p.cut ? 0.0 : -ratio * adv;
-  p.kl = 0.0;
-  if (t.has_ref) {
-    const double d = (double)t.ref_lp - (double)lp;
-    double rise;  // exp(d) - 1
-    if (fabs(d) <= 1.0) {
-      // exp(d) - d - 1 as its series, where the subtraction would cancel: the sum of
-      // d^(k - 2) / k!, k = 2 .. 11, leaves out less than 1e-8 of it
-      double s = 1.0 / 39916800.0;
-      s = fma(s, d, 1.0 / 3628800.0);
-      s = fma(s, d, 1.0 / 362880.0);
-      s = fma(s, d, 1.0 / 40320.0);
-      s = fma(s, d, 1.0 / 5040.0);
-      s = fma(s, d, 1.0 / 720.0);
-      s = fma(s, d, 1.0 / 120.0);
-      s = fma(s, d, 1.0 / 24.0);
-      s = fma(s, d, 1.0 / 6.0);
-      s = fma(s, d, 0.5);
-      p.kl = s * d * d;
-      rise = d + p.kl;
-    } else {
-      const double e = exp(d);
-      p.kl = isinf(e) ? e : e - d - 1.0;  // d itself may be infinite
-      rise = e - 1.0;
-    }
-    if (c.kl_coef != 0.0) {
-      p.value += c.kl_coef * p.kl;
-      p.slope -= c.kl_coef * rise;
-    }
-  }
+  PolicyTerm p;
+  p.cut = (t.advantage > 0.0f && above) || (t.advantage < 0.0f && below);
+  p.held = p.cut ? (above ? c.high : c.low) : ratio;
+  p.slope = p.cut ? 0.0 : -ratio * (double)t.advantage;
+  if (c.kl_coef != 0.0) p.slope -= c.kl_coef * rise;
   return p;
+}
+// Where the ratio is not cut, the unclipped term is the larger one.
+__device__ __forceinline__ double policy_value(const PolicyTerm& p, const PolicyToken& t, const PolicyClip& c,
+                                               double kl) {
+  const double value = -p.held * (double)t.advantage;
+  return c.kl_coef != 0.0 ? value + c.kl_coef * kl : value;
 }
 
 }  // namespace b2

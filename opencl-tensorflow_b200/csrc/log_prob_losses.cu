@@ -236,12 +236,13 @@ __device__ __forceinline__ void policy_part(const PolicyArgs& A, int64_t first, 
     const float w = weight_at(A.mask, A.mask_bytes, n);
     float slope = 0.0f;
     if (w != 0.0f) {
-      const PolicyTerm t =
-          policy_term(A.lp[n], PolicyToken{A.old_lp[n], A.advantages[n], has_ref ? A.ref_lp[n] : 0.0f, has_ref},
-                            A.clip);
+      const PolicyToken token{A.old_lp[n], A.advantages[n], has_ref ? A.ref_lp[n] : 0.0f, has_ref};
+      const float lp = A.lp[n];
+      const PolicyKl k = policy_kl(lp, token);
+      const PolicyTerm t = policy_term(token, A.clip, exp((double)lp - (double)token.old_lp), k.rise);
+      v[0] += (double)w * policy_value(t, token, A.clip, k.kl);
+      v[1] += (double)w * k.kl;
       slope = (float)((double)w * t.slope);
-      v[0] += (double)w * t.value;
-      v[1] += (double)w * t.kl;
       v[2] += t.cut ? (double)w : 0.0;
       v[3] += (double)w;
     }
