@@ -89,7 +89,10 @@ def policy_loss(log_probs, old_log_probs, advantages, ref_log_probs=None, mask=N
     clipped); the last two carry no gradient.  All 0 when the weights sum to 0."""
     loss, stats = step_ops.opencl_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low,
                                               clip_low if clip_high is None else clip_high, kl_coef)
-    return loss, stats[0], stats[1]
+    # The backward pass needs 1 / sum of the weights behind them: with a version counter of their own the two may be
+    # edited before it.
+    metrics = stats.data
+    return loss, metrics[0], metrics[1]
 
 
 def policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs=None, mask=None, clip_low=0.2,

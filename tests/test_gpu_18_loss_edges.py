@@ -206,3 +206,17 @@ def test_an_advantage_of_zero_has_no_gradient(otf, classes):
         near(got[0], want[0], 2 * U)
     near(parts[3], want[3], 4 * U)
     assert not parts[3][::4].any() and not fused[3][::4].any() and bool(fused[3].isfinite().all())
+
+
+def test_policy_metrics_may_be_edited_before_the_backward_pass(otf):
+    lp = (-torch.rand(300, device="cuda")).requires_grad_()
+    old, adv = lp.detach() + 0.1, torch.randn(300, device="cuda")
+
+    def loss(edit):
+        out, kl, share = otf.losses.policy_loss(lp, old, adv, ref_log_probs=old, kl_coef=0.1)
+        if edit:
+            kl /= 7
+            share.zero_()
+        return torch.autograd.grad(out, lp)[0]
+
+    assert torch.equal(loss(True), loss(False))
