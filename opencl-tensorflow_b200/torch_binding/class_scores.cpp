@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
@@ -218,17 +219,18 @@ bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_
 
 // ------------------------------------------------------------------- nodes
 
-// The losses are differentiable once: where a backward pass is itself
-// recorded, its result gets this node, which says so if it is gone through.
-struct OnceOnly : torch::autograd::Function<OnceOnly> {
-  static Tensor forward(AutogradContext*, const Tensor& grad, const Tensor&) { return grad.alias(); }
-  static tensor_list backward(AutogradContext*, tensor_list) {
-    TORCH_CHECK(false, "the gradient of a loss over class scores is differentiable once");
-  }
-};
-
-Tensor once(const Tensor& grad, const Tensor& input) {
-  return at::GradMode::is_enabled() ? OnceOnly::apply(grad, input) : grad;
+// The losses are differentiable once: where a backward pass is itself recorded,
+// its result gets a node that says so if it is gone through.  The node's edge is the
+// one of the loss's own node, to the scores or log-probabilities, so that neither
+// is kept for it.
+Tensor once(Tensor grad) {
+  if (!at::GradMode::is_enabled()) return grad;
+  const auto loss = torch::autograd::get_current_node();
+  torch::autograd::edge_list edges{loss->next_edge(0)};
+  const auto node = std::make_shared<torch::autograd::Error>(
+      "the gradient of a loss over class scores is differentiable once", std::move(edges));
+  torch::autograd::create_gradient_edge(grad, node);
+  return grad;
 }
 
 struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
@@ -256,7 +258,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
       call(true, logits, entries.token_log_probs_grad, &x, targets.data_ptr(), width(targets), floats(saved[2]),
            floats(g), out.data_ptr());
     }
-    return {once(out, logits), Tensor()};
+    return {once(out), Tensor()};
   }
 };
 
@@ -315,7 +317,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
            static_cast<int>(dtype_of(y)), ids.size(-1), data(weights), width(weights),
            ctx->saved_data["temperature"].toDouble(), floats(saved[4]), floats(grads[0]), out.data_ptr());
     }
-    return {once(out, logits), Tensor()};
+    return {once(out), Tensor()};
   }
 };
 
@@ -362,7 +364,8 @@ struct Preference : torch::autograd::Function<Preference> {
   static tensor_list forward(AutogradContext* ctx, const Tensor& log_probs, const Pairs* p) {
     Tensor slopes;
     tensor_list out = run(log_probs, *p, &slopes);
-    ctx->save_for_backward({log_probs, p->offsets, p->mask, slopes});
+    ctx->save_for_backward({p->offsets, p->mask, slopes});
+    ctx->saved_data["shape"] = log_probs.sizes();
     ctx->mark_non_differentiable({out[1]});
     ctx->set_materialize_grads(false);
     return out;
@@ -370,15 +373,15 @@ struct Preference : torch::autograd::Function<Preference> {
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    const Tensor &lp = saved[0], &offsets = saved[1], &mask = saved[2], &slopes = saved[3];
+    const Tensor &offsets = saved[0], &mask = saved[1], &slopes = saved[2];
     Tensor out;
     {
       at::NoGradGuard quiet;
-      out = new_dense(lp);
+      out = new_f32(slopes, ctx->saved_data["shape"].toIntVector());
       call(true, out, entries.preference_loss_grad, floats(grads[0]), floats(slopes), data(mask), width(mask),
            out.numel(), offsets.data_ptr(), width(offsets), slopes.numel() / 2, floats(out));
     }
-    return {once(out, lp), Tensor()};
+    return {once(out), Tensor()};
   }
 };
 
@@ -422,7 +425,7 @@ struct Policy : torch::autograd::Function<Policy> {
   static tensor_list forward(AutogradContext* ctx, const Tensor& log_probs, const Tokens* t) {
     Tensor slopes = new_dense(log_probs);
     tensor_list out = run(log_probs, *t, slopes);
-    ctx->save_for_backward({log_probs, out[1], slopes});
+    ctx->save_for_backward({out[1], slopes});
     ctx->mark_non_differentiable({out[1]});
     ctx->set_materialize_grads(false);
     return out;
@@ -430,7 +433,7 @@ struct Policy : torch::autograd::Function<Policy> {
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    const Tensor &lp = saved[0], &stats = saved[1], &slopes = saved[2];
+    const Tensor &stats = saved[0], &slopes = saved[1];
     Tensor out;
     {
       at::NoGradGuard quiet;
@@ -438,7 +441,7 @@ struct Policy : torch::autograd::Function<Policy> {
       call(true, out, entries.policy_loss_grad, floats(grads[0]), floats(stats), floats(slopes), out.numel(),
            floats(out));
     }
-    return {once(out, lp), Tensor()};
+    return {once(out), Tensor()};
   }
 };
 

@@ -220,3 +220,45 @@ def test_policy_metrics_may_be_edited_before_the_backward_pass(otf):
         return torch.autograd.grad(out, lp)[0]
 
     assert torch.equal(loss(True), loss(False))
+
+
+def test_log_probabilities_are_not_needed_after_the_loss(otf):
+    """The gradients of the token losses do not depend on them: they may be edited, and are not kept."""
+    n = 1 << 20
+    base = (-torch.rand(n, device="cuda")).requires_grad_()
+    off = cuda(0, n // 2, n)
+    adv = torch.randn(n, device="cuda")
+
+    def policy(lp):
+        return otf.losses.policy_loss(lp, adv, adv)[0]
+
+    def preference(lp):
+        return otf.losses.preference_loss(lp, off)[0]
+
+    for f in (policy, preference):
+        want, = torch.autograd.grad(f(base * 1), base)
+        lp = base.clone()
+        loss = f(lp)
+        lp.detach().zero_()
+        before = torch.cuda.memory_allocated()
+        del lp
+        assert torch.cuda.memory_allocated() <= before - 4 * n
+        assert torch.equal(torch.autograd.grad(loss, base)[0], want)
+
+
+def test_second_derivatives_are_refused(otf):
+    """Every gradient of a loss says so where it is differentiated again by its scores or log-probabilities."""
+    x = torch.randn(8, 40, device="cuda", requires_grad=True)
+    t = torch.arange(8, device="cuda")
+    off, adv = cuda(0, 4, 8), torch.randn(8, device="cuda")
+    lp = (-torch.rand(8, device="cuda")).requires_grad_()
+    for leaf, loss in ((x, lambda: otf.losses.token_log_probs(x, t).sum()),
+                       (x, lambda: otf.losses.distillation_loss(x, t[:, None], adv[:, None])),
+                       (lp, lambda: otf.losses.preference_loss(lp, off)[0]),
+                       (lp, lambda: otf.losses.policy_loss(lp, adv, adv)[0])):
+        g, = torch.autograd.grad(loss(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad((g * g).sum() + leaf.sum(), leaf)
+        g, = torch.autograd.grad((2 * loss()).exp(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(g.sum() + leaf.sum(), leaf)
