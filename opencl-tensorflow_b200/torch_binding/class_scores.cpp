@@ -220,13 +220,14 @@ bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_
 // ------------------------------------------------------------------- nodes
 
 // The losses are differentiable once: where a backward pass is itself recorded,
-// its result gets a node that says so if it is gone through.  The node's edge is the
-// one of the loss's own node, to the scores or log-probabilities, so that neither
-// is kept for it.
-Tensor once(Tensor grad) {
+// its result gets a node that says so if it is gone through.  The node has the edge
+// of the loss's own node, to the scores or log-probabilities, so that neither is
+// kept for it, and one to the upstream gradient, which the result depends on as well.
+Tensor once(Tensor grad, const Tensor& upstream) {
   if (!at::GradMode::is_enabled()) return grad;
   const auto loss = torch::autograd::get_current_node();
   torch::autograd::edge_list edges{loss->next_edge(0)};
+  if (upstream.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(upstream));
   const auto node = std::make_shared<torch::autograd::Error>(
       "the gradient of a loss over class scores is differentiable once", std::move(edges));
   torch::autograd::create_gradient_edge(grad, node);
@@ -258,7 +259,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
       call(true, logits, entries.token_log_probs_grad, &x, targets.data_ptr(), width(targets), floats(saved[2]),
            floats(g), out.data_ptr());
     }
-    return {once(out), Tensor()};
+    return {once(out, grads[0]), Tensor()};
   }
 };
 
@@ -317,7 +318,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
            static_cast<int>(dtype_of(y)), ids.size(-1), data(weights), width(weights),
            ctx->saved_data["temperature"].toDouble(), floats(saved[4]), floats(grads[0]), out.data_ptr());
     }
-    return {once(out), Tensor()};
+    return {once(out, grads[0]), Tensor()};
   }
 };
 
@@ -381,7 +382,7 @@ struct Preference : torch::autograd::Function<Preference> {
       call(true, out, entries.preference_loss_grad, floats(grads[0]), floats(slopes), data(mask), width(mask),
            out.numel(), offsets.data_ptr(), width(offsets), slopes.numel() / 2, floats(out));
     }
-    return {once(out), Tensor()};
+    return {once(out, grads[0]), Tensor()};
   }
 };
 
@@ -441,7 +442,7 @@ struct Policy : torch::autograd::Function<Policy> {
       call(true, out, entries.policy_loss_grad, floats(grads[0]), floats(stats), floats(slopes), out.numel(),
            floats(out));
     }
-    return {once(out), Tensor()};
+    return {once(out, grads[0]), Tensor()};
   }
 };
 

@@ -262,3 +262,19 @@ def test_second_derivatives_are_refused(otf):
         g, = torch.autograd.grad((2 * loss()).exp(), leaf, create_graph=True)
         with pytest.raises(RuntimeError, match="once"):
             torch.autograd.grad(g.sum() + leaf.sum(), leaf)
+
+
+def test_second_derivatives_by_what_scales_a_loss_are_refused(otf):
+    """A gradient depends on its upstream gradient too; a derivative by that must not come out without this part."""
+    x = torch.randn(8, 40, device="cuda", requires_grad=True)
+    t = torch.arange(8, device="cuda")
+    off, adv = cuda(0, 4, 8), torch.randn(8, device="cuda")
+    lp = (-torch.rand(8, device="cuda")).requires_grad_()
+    for leaf, loss in ((x, lambda: otf.losses.token_log_probs(x, t)),
+                       (x, lambda: otf.losses.distillation_loss(x, t[:, None], adv[:, None])),
+                       (lp, lambda: otf.losses.preference_loss(lp, off)[0]),
+                       (lp, lambda: otf.losses.policy_loss(lp, adv, adv)[0])):
+        scale = cuda(2.0, requires_grad=True)
+        g, = torch.autograd.grad((loss() * scale).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(g.sum() + scale.sum(), scale)
