@@ -15,7 +15,7 @@ at: whatever it holds, it adds nothing and its gradient is 0.  Scores that are N
 
 Gradients go to the scores (or log-probabilities) only: the teacher, the
 reference and old log-probabilities, advantages and weights are constants.  They are
-differentiable once.  All results are deterministic, and every call may be
+differentiable once, and backward only.  All results are deterministic, and every call may be
 captured in a CUDA graph.
 
 The ``_with_grad`` forms return the gradient of the scores with the loss, from one

@@ -125,6 +125,13 @@ const Tensor& on_cuda(py::handle h, const char* what) {
   return t;
 }
 
+// The losses have no forward-mode derivative; a tangent is refused, not dropped.
+const Tensor& no_tangent(const Tensor& t, const char* what) {
+  if (t._fw_grad(0).defined())
+    invalid(std::string(what) + " has a forward-mode tangent: the losses over class scores are differentiated backward");
+  return t;
+}
+
 // A tensor of one of the types on `like`'s device, of the given shape; contiguous.
 Tensor same(py::handle h, const char* what, c10::IntArrayRef shape, const Tensor& like, unsigned types) {
   const Tensor& t = on_cuda(h, what);
@@ -199,7 +206,7 @@ const Tensor& scores(py::handle h) {
   const Tensor& t = on_cuda(h, "logits");
   if (!(type_bit(t) & kFloats)) invalid("logits must be " + names_of(kFloats) + ", got " + text(t.scalar_type()));
   if (t.dim() < 1 || t.size(-1) < 1) invalid("logits must be [..., classes] with at least one class");
-  return t;
+  return no_tangent(t, "logits");
 }
 
 c10::IntArrayRef leading(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); }
@@ -343,7 +350,7 @@ std::tuple<Tensor, Tensor> distillation_loss_with_grad(py::handle logits, py::ha
 const Tensor& log_probs_of(py::handle h) {
   const Tensor& t = on_cuda(h, "log_probs");
   if (t.scalar_type() != at::kFloat) invalid("log_probs must be float32, got " + text(t.scalar_type()));
-  return t;
+  return no_tangent(t, "log_probs");
 }
 
 struct Pairs {

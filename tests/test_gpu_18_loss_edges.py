@@ -278,3 +278,26 @@ def test_second_derivatives_by_what_scales_a_loss_are_refused(otf):
         g, = torch.autograd.grad((loss() * scale).sum(), leaf, create_graph=True)
         with pytest.raises(RuntimeError, match="once"):
             torch.autograd.grad(g.sum() + scale.sum(), scale)
+
+
+def test_forward_mode_tangents_are_refused(otf):
+    """The losses have no forward-mode derivative: a tangent is not dropped in silence."""
+    import torch.autograd.forward_ad as fwd
+    from opencl_tf import errors
+    x, lp = torch.randn(4, 10, device="cuda"), -torch.rand(4, device="cuda")
+    t, off = torch.arange(4, device="cuda"), cuda(0, 2, 4)
+    calls = {"token_log_probs": (x, lambda a: otf.losses.token_log_probs(a, t)),
+             "distillation_loss": (x, lambda a: otf.losses.distillation_loss(a, t[:, None], lp[:, None])),
+             "distillation_loss_with_grad":
+                 (x, lambda a: otf.losses.distillation_loss_with_grad(a, t[:, None], lp[:, None])),
+             "preference_loss": (lp, lambda a: otf.losses.preference_loss(a, off)),
+             "policy_loss": (lp, lambda a: otf.losses.policy_loss(a, lp, lp)),
+             "policy_loss_with_grad": (x, lambda a: otf.losses.policy_loss_with_grad(a, t, lp, lp))}
+    for name, (primal, call) in calls.items():
+        for requires_grad in (False, True):
+            with fwd.dual_level():
+                primal = primal.detach().requires_grad_(requires_grad)
+                dual = fwd.make_dual(primal, torch.ones_like(primal))
+                with pytest.raises(errors.InvalidArgumentError, match="forward-mode"):
+                    call(dual)
+        call(primal.detach())
