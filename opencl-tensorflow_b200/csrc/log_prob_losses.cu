@@ -149,7 +149,8 @@ __device__ __forceinline__ double pair_loss(const PreferenceArgs& A, int64_t p, 
   rewards[A.pairs + p] = (float)rejected;
   slopes[p] = (float)slope;
   slopes[A.pairs + p] = (float)-slope;
-  return (1.0 - eps) * softplus(-h) + eps * softplus(h);
+  // without smoothing -log sigma(-h), infinite where the rejected answer is impossible, has no part
+  return (1.0 - eps) * softplus(-h) + (eps != 0.0 ? eps * softplus(h) : 0.0);
 }
 
 __global__ void __cluster_dims__(kSumCtas, 1, 1) __launch_bounds__(kSumThreads)

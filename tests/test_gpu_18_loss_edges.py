@@ -301,3 +301,26 @@ def test_forward_mode_tangents_are_refused(otf):
                 with pytest.raises(errors.InvalidArgumentError, match="forward-mode"):
                     call(dual)
         call(primal.detach())
+
+
+@pytest.mark.parametrize("pairs", [2, 40])  # one launch, and several
+def test_a_rejected_answer_that_the_scores_exclude(otf, pairs):
+    """Without smoothing an infinitely preferred answer costs nothing and moves nothing."""
+    lp = torch.full((2 * pairs,), -1.0, device="cuda")
+    lp[pairs] = -math.inf
+    off = torch.arange(2 * pairs + 1, device="cuda")
+    leaf = lp.clone().requires_grad_()
+    loss, chosen, rejected = otf.losses.preference_loss(leaf, off, beta=1.0)
+    near(loss, cuda((pairs - 1) * math.log(2.0) / pairs, dtype=torch.float64)[0], 2 * U)
+    assert float(rejected[0]) == -math.inf
+    grad, = torch.autograd.grad(loss, leaf)
+    want = torch.full((2 * pairs,), 0.5 / pairs, device="cuda")
+    want[:pairs] *= -1
+    want[0] = want[pairs] = 0.0
+    near(grad, want, 2 * U)
+    # with smoothing the loss is infinite, and its gradient is not
+    loss = otf.losses.preference_loss(leaf, off, beta=1.0, label_smoothing=0.1)[0]
+    assert float(loss) == math.inf and bool(torch.autograd.grad(loss, leaf)[0].isfinite().all())
+    # a chosen answer that the scores exclude: infinite, and its gradient finite
+    loss = otf.losses.preference_loss(-leaf, off, beta=1.0)[0]
+    assert float(loss) == math.inf and bool(torch.autograd.grad(loss, leaf)[0].isfinite().all())
