@@ -71,7 +71,17 @@ uint64_t pool_limit_bytes() {
   return limit;
 }
 
+// The first call on a device may be one that a CUDA graph captures: creating the
+// pool and the expiry flag is no part of any stream's work, so a capture in
+// progress need not forbid it.
+struct OutsideCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~OutsideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
 void init_device(int dev) {
+  const OutsideCapture relaxed;
   DeviceInfo& d = g_devices[dev];
   d.device = dev;
   int st = B2_OK;

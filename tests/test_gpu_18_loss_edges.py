@@ -324,3 +324,30 @@ def test_a_rejected_answer_that_the_scores_exclude(otf, pairs):
     # a chosen answer that the scores exclude: infinite, and its gradient finite
     loss = otf.losses.preference_loss(-leaf, off, beta=1.0)[0]
     assert float(loss) == math.inf and bool(torch.autograd.grad(loss, leaf)[0].isfinite().all())
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """In a process of its own, whose first calls of the library are captured ones: they replay as they run."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import torch
+from opencl_tf import losses
+torch.manual_seed(0)
+x = torch.randn(50, 6000, device="cuda")
+t = torch.arange(50, device="cuda")
+old, adv = torch.full((50,), -9.0, device="cuda"), torch.randn(50, device="cuda")
+def step():
+    return (losses.token_log_probs(x, t), *losses.policy_loss_with_grad(x, t, old, adv, mask=t > 3))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, step()))
+print("captured first")
+"""
+    package = Path(__file__).resolve().parent.parent / "opencl-tensorflow_b200"
+    done = subprocess.run([sys.executable, "-c", code], cwd=package, capture_output=True, text=True, timeout=300)
+    assert "captured first" in done.stdout, done.stderr[-2000:]
