@@ -40,14 +40,6 @@ if not _LIB_PATH.exists():
         "Build it first:\n"
         "    python opencl-tensorflow_b200/build.py")
 
-try:
-    from . import _class_scores
-except ImportError as e:
-    raise ImportError(
-        f"opencl_tf/_class_scores.so cannot be loaded ({e}).\n"
-        "Build it first:\n"
-        "    python opencl-tensorflow_b200/build.py") from e
-
 _lib = ctypes.CDLL(str(_LIB_PATH))
 
 _P = ctypes.c_void_p
@@ -611,8 +603,28 @@ def _k_upsampling_bilinear2d_grad(grad_out, input_sizes, size):
 _CLASS_SCORE_ENTRIES = ("b2_token_log_probs", "b2_token_log_probs_grad", "b2_distillation_loss",
                         "b2_distillation_loss_grad", "b2_preference_loss", "b2_preference_loss_grad", "b2_policy_loss",
                         "b2_policy_loss_grad", "b2_policy_loss_with_grad")
-_class_scores.bind([ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in _CLASS_SCORE_ENTRIES],
-                   errors.InvalidArgumentError, _check)
+
+
+def __getattr__(name: str):
+    """``_class_scores``, loaded at its first use: it is built against the installed torch, and the rest of the package
+    needs only the C library."""
+    if name != "_class_scores":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    try:
+        from . import _class_scores
+    except ImportError as e:
+        raise ImportError(
+            f"opencl_tf/_class_scores.so cannot be loaded ({e}).\n"
+            "Build it first:\n"
+            "    python opencl-tensorflow_b200/build.py") from e
+    _class_scores.bind([ctypes.cast(getattr(_lib, n), ctypes.c_void_p).value for n in _CLASS_SCORE_ENTRIES],
+                       errors.InvalidArgumentError, _check)
+    globals()[name] = _class_scores
+    return _class_scores
+
+
+def _losses_binding():
+    return globals().get("_class_scores") or __getattr__("_class_scores")
 
 
 # ------------------------------------------------------- gradient registry
@@ -822,31 +834,31 @@ def _mk_step_ops():
         return _k_mse_loss_grad(y_pred, y_true, grad_loss)
 
     def opencl_token_log_probs(logits, targets):
-        return _class_scores.token_log_probs(logits, targets)
+        return _losses_binding().token_log_probs(logits, targets)
 
     def opencl_distillation_loss(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0):
-        return _class_scores.distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature)
+        return _losses_binding().distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature)
 
     def opencl_distillation_loss_with_grad(logits, teacher_ids, teacher_logits, weights=None, temperature=1.0,
                                            grad_loss=None):
-        return _class_scores.distillation_loss_with_grad(logits, teacher_ids, teacher_logits, weights, temperature,
-                                                         grad_loss)
+        return _losses_binding().distillation_loss_with_grad(logits, teacher_ids, teacher_logits, weights, temperature,
+                                                             grad_loss)
 
     def opencl_preference_loss(log_probs, offsets, ref_log_probs=None, mask=None, beta=0.1, label_smoothing=0.0):
         """-> loss, rewards of the 2 * pairs sequences"""
-        return _class_scores.preference_loss(log_probs, offsets, ref_log_probs, mask, beta, label_smoothing)
+        return _losses_binding().preference_loss(log_probs, offsets, ref_log_probs, mask, beta, label_smoothing)
 
     def opencl_policy_loss(log_probs, old_log_probs, advantages, ref_log_probs=None, mask=None, clip_low=0.2,
                            clip_high=0.2, kl_coef=0.0):
         """-> loss, stats (mean KL, clipped share, 1 / sum of the weights)"""
-        return _class_scores.policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low,
-                                         clip_high, kl_coef)
+        return _losses_binding().policy_loss(log_probs, old_log_probs, advantages, ref_log_probs, mask, clip_low,
+                                             clip_high, kl_coef)
 
     def opencl_policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs=None, mask=None,
                                      clip_low=0.2, clip_high=0.2, kl_coef=0.0, grad_loss=None):
         """-> loss, stats (mean KL, clipped share), grad_logits"""
-        return _class_scores.policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs, mask,
-                                                   clip_low, clip_high, kl_coef, grad_loss)
+        return _losses_binding().policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_probs, mask,
+                                                       clip_low, clip_high, kl_coef, grad_loss)
 
     for k, v in list(locals().items()):
         if k.startswith("opencl_"):

@@ -42,3 +42,25 @@ def test_misaligned_row_stats_are_refused():
                        ("distillation_loss_grad", (P, 8, P, 0, 4, None, 0, 1.0, odd, P, P))):
         assert getattr(lib, "b2_" + name)(None, x, *args) == 1
         assert L._lib.b2_last_error().decode() == name + ": row_stats must be 8-byte aligned"
+
+
+def test_the_package_without_the_losses_binding():
+    """Where the compiled autograd nodes cannot be loaded, the ops, layers and optimizer are there all the same, and a
+    loss says what is missing."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import sys
+sys.modules["opencl_tf._class_scores"] = None  # importing it fails
+import torch, opencl_tf
+assert callable(opencl_tf.conv2d) and callable(opencl_tf.step_ops.opencl_mse_loss) and opencl_tf.optimizers.Adam
+try:
+    opencl_tf.losses.token_log_probs(torch.zeros(2, 3), torch.zeros(2, dtype=torch.long))
+except ImportError as e:
+    assert "build.py" in str(e)
+    print("refused")
+"""
+    package = Path(__file__).resolve().parent.parent / "opencl-tensorflow_b200"
+    done = subprocess.run([sys.executable, "-c", code], cwd=package, capture_output=True, text=True, timeout=300)
+    assert done.stdout.strip() == "refused", done.stderr[-2000:]
