@@ -59,13 +59,11 @@ def _compile(src: Path, force: bool, ptxas_v: bool) -> tuple[Path, str]:
 
 def _compile_binding(src: Path, force: bool) -> Path:
     """``opencl_tf/_<stem>.so`` from ``torch_binding/<stem>.cpp``, by the system's compiler: another one (from
-    ``CXX``, say) may link parts of a libstdc++ beside the one that torch has loaded."""
-    out = PKG / "opencl_tf" / f"_{src.stem}.so"
-    newest = max(p.stat().st_mtime for p in (src, INCLUDE / "b2_opencl_tf.h"))
-    if not force and out.exists() and out.stat().st_mtime >= newest:
-        return out
+    ``CXX``, say) may link parts of a libstdc++ beside the one that torch has loaded.  Built again when its sources
+    are newer, or with another Python, torch or command than ``_build/_<stem>.stamp`` names."""
     import torch
     from torch.utils import cpp_extension
+    out, stamp = PKG / "opencl_tf" / f"_{src.stem}.so", OBJ / f"_{src.stem}.stamp"
     cuda = Path(nvcc()).resolve().parent.parent
     includes = [a for p in cpp_extension.include_paths() for a in ("-isystem", p)]
     libs = [a for p in cpp_extension.library_paths() for a in ("-L", p)]
@@ -73,11 +71,19 @@ def _compile_binding(src: Path, force: bool) -> Path:
     cmd = [system if os.path.exists(system) else "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
            f"-DTORCH_EXTENSION_NAME=_{src.stem}", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *includes, "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"],
-           "-I", str(INCLUDE), str(src), "-o", str(out), *libs, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-           "-ltorch_python"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
+           "-I", str(INCLUDE), str(src), *libs, "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    built_with = "\n".join([sys.version, torch.__version__, *cmd])
+    newest = max(p.stat().st_mtime for p in (src, INCLUDE / "b2_opencl_tf.h"))
+    if (not force and out.exists() and out.stat().st_mtime >= newest and stamp.exists()
+            and stamp.read_text() == built_with):
+        return out
+    part = out.with_suffix(f".{os.getpid()}.part")  # a process that has the old one loaded keeps it
+    res = subprocess.run([*cmd, "-o", str(part)], capture_output=True, text=True)
     if res.returncode != 0:
+        part.unlink(missing_ok=True)
         raise RuntimeError(f"g++ failed for {src.name}:\n{res.stdout}\n{res.stderr}")
+    os.replace(part, out)
+    stamp.write_text(built_with)
     return out
 
 

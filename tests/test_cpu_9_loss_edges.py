@@ -64,3 +64,49 @@ except ImportError as e:
     package = Path(__file__).resolve().parent.parent / "opencl-tensorflow_b200"
     done = subprocess.run([sys.executable, "-c", code], cwd=package, capture_output=True, text=True, timeout=300)
     assert done.stdout.strip() == "refused", done.stderr[-2000:]
+
+
+def test_the_losses_binding_is_built_again_for_another_torch(monkeypatch, tmp_path):
+    """Its build depends on the installed torch and Python and on the command, not on file times alone; a build that
+    fails leaves the last one as it was."""
+    import importlib.util
+    import types
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location(
+        "binding_build", Path(__file__).resolve().parent.parent / "opencl-tensorflow_b200" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    monkeypatch.setattr(build, "PKG", tmp_path)
+    monkeypatch.setattr(build, "OBJ", tmp_path / "_build")
+    monkeypatch.setattr(build, "nvcc", lambda: "/usr/local/cuda/bin/nvcc")
+    (tmp_path / "_build").mkdir()
+    (tmp_path / "opencl_tf").mkdir()
+    src = tmp_path / "nodes.cpp"
+    src.write_text("")
+    runs, status = [], 0
+
+    def compiler(cmd, **_):
+        runs.append(cmd)
+        Path(cmd[cmd.index("-o") + 1]).write_text(f"build {len(runs)}")
+        return types.SimpleNamespace(returncode=status, stdout="", stderr="no")
+
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    out = build._compile_binding(src, False)
+    assert out == tmp_path / "opencl_tf" / "_nodes.so" and out.read_text() == "build 1"
+    build._compile_binding(src, False)
+    assert len(runs) == 1
+    with monkeypatch.context() as other:
+        other.setattr(torch, "__version__", "0.0.1")
+        build._compile_binding(src, False)
+        assert len(runs) == 2 and out.read_text() == "build 2"
+    build._compile_binding(src, False)
+    assert len(runs) == 3
+    build._compile_binding(src, True)
+    assert len(runs) == 4 and out.read_text() == "build 4"
+    status = 1
+    with pytest.raises(RuntimeError, match="g\\+\\+ failed"):
+        build._compile_binding(src, True)
+    assert out.read_text() == "build 4" and [p.name for p in (tmp_path / "opencl_tf").iterdir()] == ["_nodes.so"]
+    status = 0
+    build._compile_binding(src, False)
+    assert len(runs) == 5
