@@ -93,8 +93,6 @@ def build(force: bool = False, ptxas_v: bool = False, quiet: bool = True) -> Pat
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         bindings = [ex.submit(_compile_binding, s, force) for s in sorted(BINDING.glob("*.cpp"))]
         results = list(ex.map(lambda s: _compile(s, force, ptxas_v), srcs))
-        for b in bindings:
-            b.result()
     objs = [r[0] for r in results]
     if ptxas_v and not quiet:
         for _, log in results:
@@ -105,6 +103,8 @@ def build(force: bool = False, ptxas_v: bool = False, quiet: bool = True) -> Pat
         out = subprocess.run(cmd, capture_output=True, text=True)
         if out.returncode != 0:
             raise RuntimeError(f"link failed:\n{out.stdout}\n{out.stderr}")
+    for b in bindings:  # what fails here leaves the library, which needs no torch, built
+        b.result()
     if not quiet:
         print(f"built {LIB}")
     return LIB

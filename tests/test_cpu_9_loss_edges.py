@@ -110,3 +110,31 @@ def test_the_losses_binding_is_built_again_for_another_torch(monkeypatch, tmp_pa
     status = 0
     build._compile_binding(src, False)
     assert len(runs) == 5
+
+
+def test_a_binding_that_does_not_compile_leaves_the_library_built(monkeypatch, tmp_path):
+    import importlib.util
+    import types
+    from pathlib import Path
+    spec = importlib.util.spec_from_file_location(
+        "binding_build", Path(__file__).resolve().parent.parent / "opencl-tensorflow_b200" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    for name in ("OBJ", "CSRC", "BINDING"):
+        (tmp_path / name).mkdir()
+        monkeypatch.setattr(build, name, tmp_path / name)
+    monkeypatch.setattr(build, "LIB", tmp_path / "libb2ocl.so")
+    monkeypatch.setattr(build, "nvcc", lambda: "/usr/local/cuda/bin/nvcc")
+    (tmp_path / "CSRC" / "a.cu").write_text("")
+    (tmp_path / "BINDING" / "nodes.cpp").write_text("")
+
+    def compiler(cmd, **_):
+        if "nodes.cpp" in " ".join(cmd):
+            return types.SimpleNamespace(returncode=1, stdout="", stderr="no header")
+        Path(cmd[cmd.index("-o") + 1]).write_text("built")
+        return types.SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    with pytest.raises(RuntimeError, match="no header"):
+        build.build()
+    assert (tmp_path / "libb2ocl.so").read_text() == "built"
