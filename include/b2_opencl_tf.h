@@ -501,7 +501,8 @@ int b2_policy_loss_grad(b2_stream_t stream, const float* grad_loss,
 
 /* b2_policy_loss of b2_token_log_probs(logits, targets), with the gradient of
  * the scores, in one pass over them (stats has 2 elements here).  grad_loss: a
- * device float, or null for 1. */
+ * device float, or null for 1.  A row of an ignored target has log-probability 0
+ * and no gradient; only a weight of 0 keeps it out of the means. */
 int b2_policy_loss_with_grad(b2_stream_t stream, const b2_logits_t* logits,
                              const void* targets, int target_bytes,
                              const float* old_log_probs,

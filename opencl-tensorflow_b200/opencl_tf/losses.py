@@ -16,7 +16,12 @@ at: whatever it holds, it adds nothing and its gradient is 0.  Scores that are N
 Gradients go to the scores (or log-probabilities) only: the teacher, the
 reference and old log-probabilities, advantages and weights are constants.  They are
 differentiable once, and backward only.  All results are deterministic, and every call may be
-captured in a CUDA graph.
+captured in a CUDA graph (a backward pass as torch captures any: with no eager graph
+of the same leaves alive).
+
+A weighted mean divides by the sum of the call's weights.  Where ranks average their
+gradients (``TrainStep``), that is the mean over the whole batch only if the ranks' sums
+are equal; else multiply a rank's loss by its sum times the ranks over the sum of all.
 
 The ``_with_grad`` forms return the gradient of the scores with the loss, from one
 pass over the scores: ``scores.backward(grad)`` then continues the backward
@@ -43,8 +48,10 @@ def distillation_loss(logits, teacher_ids, teacher_logits, weights=None, tempera
     entries) -- a teacher's top logits.
 
     Entries whose class lies outside [0, classes) or whose logit is -inf are left
-    out; a row without entries has loss 0 and no gradient.  Entries of the same
-    class add up.  ``weights``: one per row.  0 when the weights sum to 0."""
+    out; a row without entries has loss 0 and no gradient.  A class may be repeated:
+    its entries' q add up in the gradient, and in the loss each has its own term
+    q (log q - log P), together less than that of the summed q.  ``weights``: one per
+    row.  0 when the weights sum to 0."""
     return step_ops.opencl_distillation_loss(logits, teacher_ids, teacher_logits, weights, temperature)
 
 
@@ -83,7 +90,7 @@ def policy_loss(log_probs, old_log_probs, advantages, ref_log_probs=None, mask=N
     with A = advantages, r = exp(log_probs - old_log_probs) and d =
     ref_log_probs - log_probs (no KL term without ``ref_log_probs``).
     ``clip_high`` is ``clip_low`` by default; ``mask``: which tokens count, or their
-    weights.
+    weights.  With ``kl_coef`` 0 the KL is only reported, and may be infinite.
 
     Returns (loss, mean of exp(d) - d - 1, share of the weight whose ratio is
     clipped); the last two carry no gradient.  All 0 when the weights sum to 0."""
@@ -99,7 +106,10 @@ def policy_loss_with_grad(logits, targets, old_log_probs, advantages, ref_log_pr
                           clip_high=None, kl_coef=0.0, grad_loss=None):
     """(the results of ``policy_loss`` for ``token_log_probs(logits, targets)``, the
     loss's gradient with respect to ``logits`` times ``grad_loss``) in one pass over
-    the scores: (loss, mean KL, clipped share, gradient)."""
+    the scores: (loss, mean KL, clipped share, gradient).
+
+    A target outside [0, classes) is a token of log-probability 0 without gradient:
+    unless ``mask`` leaves it out, its ratio exp(-old_log_probs) counts in the means."""
     loss, stats, grad = step_ops.opencl_policy_loss_with_grad(
         logits, targets, old_log_probs, advantages, ref_log_probs, mask, clip_low,
         clip_low if clip_high is None else clip_high, kl_coef, grad_loss)

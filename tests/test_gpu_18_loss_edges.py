@@ -351,3 +351,46 @@ print("captured first")
     package = Path(__file__).resolve().parent.parent / "opencl-tensorflow_b200"
     done = subprocess.run([sys.executable, "-c", code], cwd=package, capture_output=True, text=True, timeout=300)
     assert "captured first" in done.stdout, done.stderr[-2000:]
+
+
+def test_the_losses_as_they_are_called_in_a_program(otf):
+    """Log-probabilities of a view to a preference loss, a policy step in one call with ignored targets, a captured
+    distillation step: what each returns."""
+    from opencl_tf import losses
+    from opencl_tf.train import TrainStep
+    torch.manual_seed(5)
+    scores = torch.randn(4, 9, 50, device="cuda", requires_grad=True)
+    tokens = torch.randint(0, 50, (4, 9), device="cuda")
+    answer = torch.rand(4, 8, device="cuda") > 0.2
+    offsets, ref = cuda(0, 8, 16, 24, 32), -torch.rand(32, device="cuda")
+    lp = losses.token_log_probs(scores[:, :-1], tokens[:, 1:])
+    loss, chosen, rejected = losses.preference_loss(lp.flatten(), offsets, ref_log_probs=ref, mask=answer.flatten())
+    loss.backward()
+    assert chosen.shape == rejected.shape == (2,) and bool(scores.grad.isfinite().all()) and bool(scores.grad.any())
+    scores.grad = None
+    tokens[:, 0] = -100
+    old, advantages = -torch.rand(4, 9, device="cuda"), torch.randn(4, 9, device="cuda")
+    loss, kl, clipped, grad = losses.policy_loss_with_grad(scores, tokens, old, advantages, ref_log_probs=old,
+                                                           mask=tokens >= 0, kl_coef=0.02)
+    scores.backward(grad)
+    assert loss.shape == kl.shape == clipped.shape == () and torch.equal(scores.grad, grad)
+    assert not grad[:, 0].any() and bool(grad[:, 1:].any(-1).all())
+    # without the mask the ignored targets count, with log-probability 0
+    lp = losses.token_log_probs(scores.detach(), tokens)
+    assert not lp[:, 0].any()
+    for mask in (None, tokens >= 0):
+        got = losses.policy_loss_with_grad(scores, tokens, old, advantages, ref_log_probs=old, mask=mask, kl_coef=0.02)
+        keep = slice(0 if mask is None else 1, None)
+        want = policy_definition(lp[:, keep].flatten(), old[:, keep].flatten(), advantages[:, keep].flatten(),
+                                 old[:, keep].flatten(), kl_coef=0.02)
+        # the log-probability of the fused pass may be two roundings off: 4 U of at most |lp| < 16, moving a term by
+        # at most its ratio times its advantage and the KL's slope
+        near(got[0], want[0], 2 * U, 64 * U * float(want[3].abs().sum() + want[2] * advantages.abs().max()))
+        near(got[1], want[1], 2 * U, 64 * U * float(torch.expm1(old.double() - lp.double()).abs().max()))
+        near(got[2], want[2], 2 * U)
+    torch.manual_seed(0)
+    model = _Head().cuda()
+    step = TrainStep(model, lr=1e-3, loss=lambda out, t: losses.distillation_loss(out, t[0], t[1], temperature=2.0))
+    top = torch.randn(16, 33, device="cuda").topk(4, 1)
+    loss = step(torch.randn(16, 12, device="cuda"), (top.indices, top.values))
+    assert math.isfinite(float(loss))
