@@ -394,3 +394,61 @@ def test_the_losses_as_they_are_called_in_a_program(otf):
     top = torch.randn(16, 33, device="cuda").topk(4, 1)
     loss = step(torch.randn(16, 12, device="cuda"), (top.indices, top.values))
     assert math.isfinite(float(loss))
+
+
+# 8 lanes a row, a warp, a CTA, a cluster
+@pytest.mark.parametrize("rows,classes,dtype", [(30011, 37, "f32"), (29000, 1500, "bf16"), (15000, 5003, "f16"),
+                                                (1200, 2100, "f32"), (700, 16000, "bf16"), (160, 60000, "f16"),
+                                                (9, 200000, "f32")])
+def test_policy_loss_with_grad_of_many_rows(otf, rows, classes, dtype):
+    """Loss and gradient against the definition in 64 bits.  The log-probability l that the ratio is taken from is off by
+    u (3 D + 4 + c) + 2 u |l| + u: D = sum p |x - m|, c additions and merges that follow one another in a row's sum
+    (at most 32, then an eighth of a row's values in batches of 32, then 61 in merging)."""
+    dt = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    eps = torch.finfo(dt).eps / 2
+    tiny = {"f32": 2.0 ** -126, "f16": 2.0 ** -25, "bf16": 2.0 ** -126}[dtype]
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = (3 * torch.randn(rows, classes, generator=g, device="cuda")).to(dt)
+    t = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+    t[::7] = -100  # counted, with log-probability 0 and no gradient
+    z = torch.log_softmax(x.double(), 1)
+    ignored = t < 0
+    at = t.clamp(min=0)[:, None]
+    lp = torch.where(ignored, torch.zeros_like(z[:, 0]), z.gather(1, at)[:, 0])
+    ratio = torch.rand(rows, generator=g, device="cuda") * 0.15 + torch.where(
+        torch.rand(rows, generator=g, device="cuda") < 0.5, 0.9, 1.5)  # away from the borders 0.8 and 1.28
+    old = (lp - ratio.double().log()).float()
+    ref = (lp + 0.3 * torch.randn(rows, generator=g, device="cuda")).float()
+    adv = torch.randn(rows, generator=g, device="cuda")
+    w = torch.rand(rows, generator=g, device="cuda") + 0.1
+    w[rows // 2] = 0.0
+    scale, coef = 4096.0, 0.05
+    loss, kl, share, grad = otf.losses.policy_loss_with_grad(
+        x, t, old, adv, ref_log_probs=ref, mask=w, clip_low=0.2, clip_high=0.28, kl_coef=coef, grad_loss=cuda(scale)[0])
+
+    r = torch.exp(lp - old.double())
+    a, wd = adv.double(), w.double()
+    cut = ((a > 0) & (r > 1.28)) | ((a < 0) & (r < 0.8))
+    d = ref.double() - lp
+    k3 = torch.expm1(d) - d
+    value = -torch.where(cut, r.clamp(0.8, 1.28), r) * a + coef * k3
+    slope = torch.where(cut, torch.zeros_like(r), -r * a) - coef * torch.expm1(d)
+    share_w = wd / wd.sum()
+    p = z.exp()
+    away = torch.where(p > 0, x.double().amax(1, keepdim=True) - x.double(), torch.zeros_like(p))
+    rel_s = U * (3 * (p * away).sum(1) + 4 + 93 + classes / 256)
+    lp_off = torch.where(ignored, torch.zeros_like(lp), rel_s + 2 * U * lp.abs() + U)
+    # a token's value moves with its log-probability by its slope, which itself moves by at most r |a| + coef exp(d)
+    bend = r * a.abs() + coef * torch.exp(d)
+    near(loss, (share_w * value).sum(), U, float((share_w * (slope.abs() + bend * lp_off) * lp_off).sum()))
+    near(kl, (share_w * k3).sum(), U + 2e-8, float((share_w * (torch.expm1(d).abs() + torch.exp(d) * lp_off) * lp_off).sum()))
+    near(share, (share_w * cut).sum(), U)
+    factor = torch.where(ignored, torch.zeros_like(slope), scale * share_w * slope)[:, None]
+    hot = torch.zeros_like(p).scatter_(1, at, 1.0)
+    want = factor * (hot - p)
+    moved = (scale * share_w * bend * lp_off * ~ignored)[:, None] * (hot - p).abs()
+    # p: 3 u |x - m| and 8 u of its own beside s; the difference, the factor's roundings, the store
+    tol = factor.abs() * (p * (rel_s[:, None] + U * (3 * away + 8)) + 2 * U) + want.abs() * (6 * U + eps) + tiny
+    off = (grad.double() - want).abs()
+    assert bool((off <= tol + moved).all()), float((off - tol - moved).max())
+    assert not grad[ignored].any() and not grad[rows // 2].any()
