@@ -13,6 +13,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/custom_class.h>
 #include <torch/extension.h>
 
 #include <cstring>
@@ -227,13 +228,22 @@ bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_
 // ------------------------------------------------------------------- nodes
 
 // The losses are differentiable once: where a backward pass is itself recorded,
-// its result gets a node that says so if it is gone through.  The node has the edge
-// of the loss's own node, to the scores or log-probabilities, so that neither is
-// kept for it, and one to the upstream gradient, which the result depends on as well.
-Tensor once(Tensor grad, const Tensor& upstream) {
+// its result gets a node that says so if it is gone through.  The node has an edge
+// to the loss's scores or log-probabilities, remembered by the loss's own node so
+// that neither tensor is kept for it, and one to the upstream gradient, which the
+// result depends on as well.
+struct InputEdge : torch::CustomClassHolder {
+  explicit InputEdge(const Tensor& input) : edge(torch::autograd::impl::gradient_edge(input)) {}
+  torch::autograd::Edge edge;
+};
+
+void remember(AutogradContext* ctx, const Tensor& input) {
+  ctx->saved_data["input"] = c10::IValue::make_capsule(c10::make_intrusive<InputEdge>(input));
+}
+
+Tensor once(AutogradContext* ctx, Tensor grad, const Tensor& upstream) {
   if (!at::GradMode::is_enabled()) return grad;
-  const auto loss = torch::autograd::get_current_node();
-  torch::autograd::edge_list edges{loss->next_edge(0)};
+  torch::autograd::edge_list edges{static_cast<InputEdge*>(ctx->saved_data["input"].toCapsule().get())->edge};
   if (upstream.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(upstream));
   const auto node = std::make_shared<torch::autograd::Error>(
       "the gradient of a loss over class scores is differentiable once", std::move(edges));
@@ -252,6 +262,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
     Tensor stats = new_f32(logits, {targets->numel(), 2});
     Tensor out = run(logits, *targets, stats);
     ctx->save_for_backward({logits, *targets, stats});
+    remember(ctx, logits);
     return out;
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
@@ -266,7 +277,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
       call(true, logits, entries.token_log_probs_grad, &x, targets.data_ptr(), width(targets), floats(saved[2]),
            floats(g), out.data_ptr());
     }
-    return {once(out, grads[0]), Tensor()};
+    return {once(ctx, out, grads[0]), Tensor()};
   }
 };
 
@@ -311,6 +322,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
     Tensor loss = run(logits, *t, stats, Tensor(), Tensor());
     ctx->save_for_backward({logits, t->ids, t->y, t->weights, stats});
     ctx->saved_data["temperature"] = t->temperature;
+    remember(ctx, logits);
     return loss;
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
@@ -325,7 +337,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
            static_cast<int>(dtype_of(y)), ids.size(-1), data(weights), width(weights),
            ctx->saved_data["temperature"].toDouble(), floats(saved[4]), floats(grads[0]), out.data_ptr());
     }
-    return {once(out, grads[0]), Tensor()};
+    return {once(ctx, out, grads[0]), Tensor()};
   }
 };
 
@@ -374,6 +386,7 @@ struct Preference : torch::autograd::Function<Preference> {
     tensor_list out = run(log_probs, *p, &slopes);
     ctx->save_for_backward({p->offsets, p->mask, slopes});
     ctx->saved_data["shape"] = log_probs.sizes();
+    remember(ctx, log_probs);
     ctx->mark_non_differentiable({out[1]});
     ctx->set_materialize_grads(false);
     return out;
@@ -389,7 +402,7 @@ struct Preference : torch::autograd::Function<Preference> {
       call(true, out, entries.preference_loss_grad, floats(grads[0]), floats(slopes), data(mask), width(mask),
            out.numel(), offsets.data_ptr(), width(offsets), slopes.numel() / 2, floats(out));
     }
-    return {once(out, grads[0]), Tensor()};
+    return {once(ctx, out, grads[0]), Tensor()};
   }
 };
 
@@ -434,6 +447,7 @@ struct Policy : torch::autograd::Function<Policy> {
     Tensor slopes = new_dense(log_probs);
     tensor_list out = run(log_probs, *t, slopes);
     ctx->save_for_backward({out[1], slopes});
+    remember(ctx, log_probs);
     ctx->mark_non_differentiable({out[1]});
     ctx->set_materialize_grads(false);
     return out;
@@ -449,7 +463,7 @@ struct Policy : torch::autograd::Function<Policy> {
       call(true, out, entries.policy_loss_grad, floats(grads[0]), floats(stats), floats(slopes), out.numel(),
            floats(out));
     }
-    return {once(out, grads[0]), Tensor()};
+    return {once(ctx, out, grads[0]), Tensor()};
   }
 };
 

@@ -452,3 +452,28 @@ def test_policy_loss_with_grad_of_many_rows(otf, rows, classes, dtype):
     off = (grad.double() - want).abs()
     assert bool((off <= tol + moved).all()), float((off - tol - moved).max())
     assert not grad[ignored].any() and not grad[rows // 2].any()
+
+
+def test_a_loss_node_called_by_itself(otf):
+    """The node of a loss, called outside of a backward pass, gives the gradient that a backward pass gives; recorded,
+    it refuses to be differentiated again."""
+    x = torch.randn(8, 40, device="cuda", requires_grad=True)
+    t = torch.arange(8, device="cuda")
+    off, adv = cuda(0, 4, 8), torch.randn(8, device="cuda")
+    lp = (-torch.rand(8, device="cuda")).requires_grad_()
+    for leaf, loss in ((x, lambda: otf.losses.token_log_probs(x, t)),
+                       (x, lambda: otf.losses.distillation_loss(x, t[:, None], adv[:, None])),
+                       (lp, lambda: otf.losses.preference_loss(lp, off)[0]),
+                       (lp, lambda: otf.losses.policy_loss(lp, adv, adv)[0])):
+        out = loss()
+        up = torch.ones_like(out)
+        want, = torch.autograd.grad(loss(), leaf, up)
+        for recorded in (False, True):
+            out = loss()
+            with torch.set_grad_enabled(recorded):
+                got = out.grad_fn(*(up, None)[:len(out.grad_fn._input_metadata)])  # a second result has no gradient
+            got = got[0] if isinstance(got, tuple) else got
+            assert torch.equal(got, want) and got.requires_grad == recorded
+            if recorded:
+                with pytest.raises(RuntimeError, match="once"):
+                    torch.autograd.grad(got.sum() + leaf.sum(), leaf)
