@@ -302,6 +302,7 @@ def _copies(buffers, given, what: str) -> list:
     return list(zip(bs, ts))
 
 
+@torch.no_grad()
 def _copy(pairs, non_blocking: bool = False) -> None:
     for b, t in pairs:
         if t.data_ptr() != b.data_ptr():
@@ -394,8 +395,7 @@ class TrainStep:
     def _capture(self, x, y):
         self.static_x = torch.empty_like(x)
         self.static_y = _buffers_like(y)
-        self.static_x.copy_(x)
-        _copy(_copies(self.static_y, y, "targets"))
+        _copy(_copies(self.static_x, x, "input") + _copies(self.static_y, y, "targets"))
         side = torch.cuda.Stream(device=x.device)
         side.wait_stream(torch.cuda.current_stream(x.device))
         with torch.cuda.stream(side):
@@ -431,8 +431,7 @@ class TrainStep:
         if self.graph1 is None:
             self.static_x1 = torch.empty_like(self.static_x)
             self.static_y1 = _buffers_like(self.static_y)
-            self.static_x1.copy_(self.static_x)
-            _copy(_copies(self.static_y1, self.static_y, "targets"))
+            _copy(_copies(self.static_x1, self.static_x, "input") + _copies(self.static_y1, self.static_y, "targets"))
             torch.cuda.current_stream(self.static_x.device).synchronize()
             self.graph1 = torch.cuda.CUDAGraph()
             self.zero_grad()

@@ -138,3 +138,14 @@ def test_a_binding_that_does_not_compile_leaves_the_library_built(monkeypatch, t
     with pytest.raises(RuntimeError, match="no header"):
         build.build()
     assert (tmp_path / "libb2ocl.so").read_text() == "built"
+
+
+def test_a_captured_steps_buffers_stay_out_of_autograd():
+    """Targets that a recorded network computed (a teacher's logits) are values: the buffers keep no graph of them, which
+    would grow from step to step."""
+    from opencl_tf import train
+    teacher = torch.nn.Linear(3, 5)
+    buffers = (torch.zeros(4, 5), torch.zeros(4, 5))
+    for _ in range(2):
+        train._copy(train._copies(buffers, (teacher(torch.randn(4, 3)), torch.randn(4, 5)), "targets"))
+        assert not any(b.requires_grad for b in buffers)
