@@ -228,28 +228,35 @@ bool records(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_
 // ------------------------------------------------------------------- nodes
 
 // The losses are differentiable once: where a backward pass is itself recorded,
-// its result gets a node that says so if it is gone through.  The node has an edge
-// to the loss's scores or log-probabilities, remembered by the loss's own node so
-// that neither tensor is kept for it, and one to the upstream gradient, which the
-// result depends on as well.
-struct InputEdge : torch::CustomClassHolder {
-  explicit InputEdge(const Tensor& input) : edge(torch::autograd::impl::gradient_edge(input)) {}
-  torch::autograd::Edge edge;
-};
-
-void remember(AutogradContext* ctx, const Tensor& input) {
-  ctx->saved_data["input"] = c10::IValue::make_capsule(c10::make_intrusive<InputEdge>(input));
-}
-
-Tensor once(AutogradContext* ctx, Tensor grad, const Tensor& upstream) {
-  if (!at::GradMode::is_enabled()) return grad;
-  torch::autograd::edge_list edges{static_cast<InputEdge*>(ctx->saved_data["input"].toCapsule().get())->edge};
+// its result gets a node that says so if it is gone through, with an edge to the
+// loss's scores or log-probabilities and one to the upstream gradient, on which the
+// result depends as well.
+Tensor once(Tensor grad, const torch::autograd::Edge& input, const Tensor& upstream) {
+  torch::autograd::edge_list edges{input};
   if (upstream.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(upstream));
   const auto node = std::make_shared<torch::autograd::Error>(
       "the gradient of a loss over class scores is differentiable once", std::move(edges));
   torch::autograd::create_gradient_edge(grad, node);
   return grad;
 }
+
+Tensor once(const Tensor& grad, const Tensor& input, const Tensor& upstream) {
+  return at::GradMode::is_enabled() ? once(grad, torch::autograd::impl::gradient_edge(input), upstream) : grad;
+}
+
+// What a gradient needs of log-probabilities that need not be kept for it.
+struct Origin : torch::CustomClassHolder {
+  explicit Origin(const Tensor& t) : edge(torch::autograd::impl::gradient_edge(t)), shape(t.sizes().vec()) {}
+  torch::autograd::Edge edge;
+  std::vector<int64_t> shape;
+
+  static void keep(AutogradContext* ctx, const Tensor& t) {
+    ctx->saved_data["origin"] = c10::IValue::make_capsule(c10::make_intrusive<Origin>(t));
+  }
+  static c10::intrusive_ptr<Origin> of(AutogradContext* ctx) {
+    return c10::static_intrusive_pointer_cast<Origin>(ctx->saved_data["origin"].toCapsule());
+  }
+};
 
 struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
   static Tensor run(const Tensor& logits, const Tensor& targets, const Tensor& stats) {
@@ -262,7 +269,6 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
     Tensor stats = new_f32(logits, {targets->numel(), 2});
     Tensor out = run(logits, *targets, stats);
     ctx->save_for_backward({logits, *targets, stats});
-    remember(ctx, logits);
     return out;
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
@@ -277,7 +283,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
       call(true, logits, entries.token_log_probs_grad, &x, targets.data_ptr(), width(targets), floats(saved[2]),
            floats(g), out.data_ptr());
     }
-    return {once(ctx, out, grads[0]), Tensor()};
+    return {once(out, logits, grads[0]), Tensor()};
   }
 };
 
@@ -322,7 +328,6 @@ struct Distillation : torch::autograd::Function<Distillation> {
     Tensor loss = run(logits, *t, stats, Tensor(), Tensor());
     ctx->save_for_backward({logits, t->ids, t->y, t->weights, stats});
     ctx->saved_data["temperature"] = t->temperature;
-    remember(ctx, logits);
     return loss;
   }
   static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
@@ -337,7 +342,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
            static_cast<int>(dtype_of(y)), ids.size(-1), data(weights), width(weights),
            ctx->saved_data["temperature"].toDouble(), floats(saved[4]), floats(grads[0]), out.data_ptr());
     }
-    return {once(ctx, out, grads[0]), Tensor()};
+    return {once(out, logits, grads[0]), Tensor()};
   }
 };
 
@@ -385,8 +390,7 @@ struct Preference : torch::autograd::Function<Preference> {
     Tensor slopes;
     tensor_list out = run(log_probs, *p, &slopes);
     ctx->save_for_backward({p->offsets, p->mask, slopes});
-    ctx->saved_data["shape"] = log_probs.sizes();
-    remember(ctx, log_probs);
+    Origin::keep(ctx, log_probs);
     ctx->mark_non_differentiable({out[1]});
     ctx->set_materialize_grads(false);
     return out;
@@ -395,14 +399,15 @@ struct Preference : torch::autograd::Function<Preference> {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
     const Tensor &offsets = saved[0], &mask = saved[1], &slopes = saved[2];
+    const auto origin = Origin::of(ctx);
     Tensor out;
     {
       at::NoGradGuard quiet;
-      out = new_f32(slopes, ctx->saved_data["shape"].toIntVector());
+      out = new_f32(slopes, origin->shape);
       call(true, out, entries.preference_loss_grad, floats(grads[0]), floats(slopes), data(mask), width(mask),
            out.numel(), offsets.data_ptr(), width(offsets), slopes.numel() / 2, floats(out));
     }
-    return {once(ctx, out, grads[0]), Tensor()};
+    return {at::GradMode::is_enabled() ? once(out, origin->edge, grads[0]) : out, Tensor()};
   }
 };
 
@@ -447,7 +452,7 @@ struct Policy : torch::autograd::Function<Policy> {
     Tensor slopes = new_dense(log_probs);
     tensor_list out = run(log_probs, *t, slopes);
     ctx->save_for_backward({out[1], slopes});
-    remember(ctx, log_probs);
+    Origin::keep(ctx, log_probs);
     ctx->mark_non_differentiable({out[1]});
     ctx->set_materialize_grads(false);
     return out;
@@ -456,6 +461,7 @@ struct Policy : torch::autograd::Function<Policy> {
     if (!grads[0].defined()) return {Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
     const Tensor &stats = saved[0], &slopes = saved[1];
+    const auto origin = Origin::of(ctx);
     Tensor out;
     {
       at::NoGradGuard quiet;
@@ -463,7 +469,7 @@ struct Policy : torch::autograd::Function<Policy> {
       call(true, out, entries.policy_loss_grad, floats(grads[0]), floats(stats), floats(slopes), out.numel(),
            floats(out));
     }
-    return {once(ctx, out, grads[0]), Tensor()};
+    return {at::GradMode::is_enabled() ? once(out, origin->edge, grads[0]) : out, Tensor()};
   }
 };
 
